@@ -78,6 +78,12 @@ SIGNATURES = {
     "eg2_launch_gate_quant": (i32, [vp, vp]),
     "eg2_launch_gelu_mul": (i32, [vp, vp]),
     "eg2_launch_pool_l2": (i32, [vp, vp]),
+    "eg2_launch_embed_rows": (i32, [vp, vp]),
+    "eg2_embed_rows_grad_workspace": (C.c_uint64, [u32, u32]),
+    "eg2_launch_embed_rows_grad": (i32, [vp, vp]),
+    "eg2_launch_qkv_norm_rope": (i32, [vp, vp]),
+    "eg2_qkv_norm_rope_grad_workspace": (C.c_uint64, [u32, u32, u32, u32]),
+    "eg2_launch_qkv_norm_rope_grad": (i32, [vp, vp]),
     "eg2_repack_q8": (i32, [vp, u32, u32, vp, vp, vp]),
     "eg2_read_error": (i32, []),
     "eg2_clear_error": (None, []),
@@ -198,6 +204,36 @@ class EgPoolL2(C.Structure):
     _fields_ = [("out", P), ("y", P), ("offsets", P), ("batch", u32), ("width", u32)]
 
 
+i64, u64 = C.c_int64, C.c_uint64
+P2, P3, Strides3 = P * 2, P * 3, (i64 * 2) * 3
+
+
+class EgEmbedRows(C.Structure):
+    _fields_ = [("out", P), ("table", P), ("ids", P), ("out_stride", i64), ("table_stride", i64), ("n", u32),
+                ("vocab", u32), ("d", u32), ("out_type", u32), ("table_type", u32), ("scale", f32)]
+
+
+class EgEmbedRowsGrad(C.Structure):
+    _fields_ = [("dtable", P), ("dout", P), ("ids", P), ("workspace", P), ("workspace_bytes", u64),
+                ("dtable_stride", i64), ("dout_stride", i64), ("n", u32), ("vocab", u32), ("d", u32),
+                ("dtable_type", u32), ("dout_type", u32), ("scale", f32), ("accumulate", u32)]
+
+
+class EgQkvNormRope(C.Structure):
+    _fields_ = [("out", P3), ("x", P3), ("weight", P2), ("rope_cos", P), ("rope_sin", P), ("pos", P),
+                ("out_stride", Strides3), ("x_stride", Strides3), ("n", u32), ("q_heads", u32), ("k_heads", u32),
+                ("v_heads", u32), ("d", u32), ("positions", u32), ("type", u32), ("weight_type", u32), ("eps", f32)]
+
+
+class EgQkvNormRopeGrad(C.Structure):
+    _fields_ = [("dx", P3), ("dweight", P2), ("dout", P3), ("x", P3), ("weight", P2), ("rope_cos", P),
+                ("rope_sin", P), ("pos", P), ("workspace", P), ("workspace_bytes", u64), ("dx_stride", Strides3),
+                ("dout_stride", Strides3), ("x_stride", Strides3), ("n", u32), ("q_heads", u32), ("k_heads", u32),
+                ("v_heads", u32), ("d", u32), ("positions", u32), ("type", u32), ("weight_type", u32), ("eps", f32),
+                ("accumulate", u32)]
+
+
 STRUCTS = {c.__name__: c for c in (EgGather, EgMM, EgNorm, EgRope, EgAttention, EgElement, EgPool, EgNormResidual,
                                    EgNormRope, EgEmbed, EgPleProj, EgNormQuant, EgQ8MM, EgQ8GeGLU, EgQkvPost, EgAttentionF16,
-                                   EgPostAdd, EgGateQuant, EgGeluMul, EgPoolL2)}
+                                   EgPostAdd, EgGateQuant, EgGeluMul, EgPoolL2, EgEmbedRows, EgEmbedRowsGrad, EgQkvNormRope,
+                                   EgQkvNormRopeGrad)}

@@ -520,3 +520,5 @@ int eg2_selftest_wait_timeout(void *s) {
 int eg2_read_error(void) { return read_device_error(); }
 void eg2_clear_error(void) { clear_device_error(); }
 }
+
+#include "rowops_abi.cuh"

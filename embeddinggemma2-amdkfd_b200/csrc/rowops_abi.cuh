@@ -1,0 +1,306 @@
+// Launchers and C entry points (include/eg2_ops.h, part 3) of the typed row
+// operators: argument checks, the choice of a kernel by type, width and
+// alignment, and workspace layout.  Included once, at the end of kernels.cu.
+#pragma once
+#include "embedrows.cuh"
+#include "qkvnorm.cuh"
+
+namespace eg2 {
+
+static inline int type_size(unsigned t) { return t == EG_F32 ? 4 : t == EG_F16 || t == EG_BF16 ? 2 : 0; }
+static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static inline int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
+
+// f(type tag) for an element type; cudaErrorInvalidValue for any other number.
+template <typename T>
+struct Tag {
+    using type = T;
+};
+template <typename F>
+static cudaError_t by_type(unsigned t, F f) {
+    switch (t) {
+        case EG_F32: return f(Tag<float>{});
+        case EG_F16: return f(Tag<__half>{});
+        case EG_BF16: return f(Tag<__nv_bfloat16>{});
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+// ---------------------------------------------------------------- embed_rows
+static cudaError_t embed_rows(const EgEmbedRows &a, cudaStream_t s) {
+    const int so = type_size(a.out_type), st = type_size(a.table_type);
+    if (!so || !st || !a.d || a.d > (1u << 20) || a.n > 0x7fffffffu || a.vocab > 0x7ffffffeu)
+        return cudaErrorInvalidValue;
+    if (!a.n) return cudaSuccess;
+    if (!a.out || !a.ids || (a.vocab && !a.table) || (a.n > 1 && a.out_stride < (int64_t)a.d) ||
+        (a.vocab > 1 && a.table_stride < (int64_t)a.d))
+        return cudaErrorInvalidValue;
+    const EmbedRowsParams p{a.out, a.table, a.ids, a.out_stride, a.table_stride, int(a.n), int(a.vocab), int(a.d),
+                            a.scale};
+    const bool wide = a.d % 8 == 0 && aligned16(a.out) && aligned16(a.table) &&
+                      (a.n == 1 || a.out_stride * so % 16 == 0) && (a.vocab < 2 || a.table_stride * st % 16 == 0);
+    return by_type(a.table_type, [&](auto ti) {
+        return by_type(a.out_type, [&](auto to) {
+            using TI = typename decltype(ti)::type;
+            using TO = typename decltype(to)::type;
+            // Four rows a warp while that still fills the GPU, else one.
+            const bool four = a.n >= 16384;
+            const dim3 grid(ceil_div(a.n, four ? 32 : 8));
+            if (wide)
+                return four ? launch_pdl(embed_rows_kernel<TI, TO, 8, 4>, grid, dim3(256), 0, s, p)
+                            : launch_pdl(embed_rows_kernel<TI, TO, 8, 1>, grid, dim3(256), 0, s, p);
+            return four ? launch_pdl(embed_rows_kernel<TI, TO, 1, 4>, grid, dim3(256), 0, s, p)
+                        : launch_pdl(embed_rows_kernel<TI, TO, 1, 1>, grid, dim3(256), 0, s, p);
+        });
+    });
+}
+
+// Workspace: two (key, token) arrays, the digit histogram, and the head and tail
+// parts of every chunk.
+struct EmbedGradLayout {
+    int tiles, subtiles, chunk, chunks;
+    size_t key[2], tok[2], hist, head, tail, total;
+};
+static EmbedGradLayout embed_grad_layout(unsigned n, unsigned d) {
+    EmbedGradLayout L{};
+    // Short chunks while the batch is small, for more warps; long ones leave fewer parts to join.
+    L.chunk = n >= 32768 ? 32 : 8;
+    L.chunks = ceil_div(n, L.chunk);
+    L.subtiles = ceil_div(n, (long long)EmbedSort::SUB * EmbedSort::MAX_TILES);
+    if (L.subtiles < 1) L.subtiles = 1;
+    L.tiles = ceil_div(n, (long long)EmbedSort::SUB * L.subtiles);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    for (int i = 0; i < 2; ++i) L.key[i] = take(size_t(n) * 4), L.tok[i] = take(size_t(n) * 4);
+    L.hist = take(size_t(L.tiles) * EmbedSort::MAX_BINS * 4);
+    L.head = take(size_t(L.chunks) * d * 4);
+    L.tail = take(size_t(L.chunks) * d * 4);
+    L.total = at;
+    return L;
+}
+
+static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
+    const int sw = type_size(a.dtable_type), sg = type_size(a.dout_type);
+    if (!sw || !sg || !a.d || a.d > (1u << 20) || a.n > 0x7fffffffu || a.vocab > 0x7ffffffeu)
+        return cudaErrorInvalidValue;
+    if (!a.vocab || (!a.n && a.accumulate)) return cudaSuccess;
+    if (!a.dtable || (a.vocab > 1 && a.dtable_stride < (int64_t)a.d)) return cudaErrorInvalidValue;
+    const long long stride = a.vocab > 1 ? a.dtable_stride : a.d;
+    if (!a.n)
+        return cudaMemset2DAsync(a.dtable, size_t(stride) * sw, 0, size_t(a.d) * sw, a.vocab, s);
+    const EmbedGradLayout L = embed_grad_layout(a.n, a.d);
+    if (!a.dout || !a.ids || !a.workspace || a.workspace_bytes < L.total ||
+        (reinterpret_cast<uintptr_t>(a.workspace) & 255) || a.dout_stride < 0)
+        return cudaErrorInvalidValue;
+    uint8_t *ws = static_cast<uint8_t *>(a.workspace);
+    unsigned *key[2] = {reinterpret_cast<unsigned *>(ws + L.key[0]), reinterpret_cast<unsigned *>(ws + L.key[1])};
+    int *tok[2] = {reinterpret_cast<int *>(ws + L.tok[0]), reinterpret_cast<int *>(ws + L.tok[1])};
+
+    // Keys are 0 .. vocab (padding last); equal digits over as few passes as cover them.
+    int key_bits = 1;
+    while (key_bits < 31 && (a.vocab >> key_bits)) ++key_bits;
+    const int passes = ceil_div(key_bits, EmbedSort::MAX_BITS), bits = ceil_div(key_bits, passes);
+    EmbedSortParams q{};
+    q.hist = reinterpret_cast<unsigned *>(ws + L.hist);
+    q.n = int(a.n), q.vocab = int(a.vocab), q.tiles = L.tiles, q.subtiles = L.subtiles, q.bits = bits;
+    if (!a.accumulate) {
+        // The table is cleared by CTAs beside the sort's, a share of its rows in each of its launches.
+        q.fill = static_cast<unsigned char *>(a.dtable);
+        q.fill_stride_bytes = stride * sw, q.fill_width_bytes = int(a.d) * sw;
+        const long long want = ceil_div((long long)a.vocab * a.d * sw, 2 * passes * 65536ll);
+        q.fill_ctas = int(want < 1 ? 1 : want > 4 * sm_count() ? 4 * sm_count() : want);
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        q.ids = pass ? nullptr : a.ids;
+        q.key_in = key[pass & 1], q.tok_in = tok[pass & 1];
+        q.key_out = key[(pass + 1) & 1], q.tok_out = tok[(pass + 1) & 1];
+        q.shift = pass * bits;
+        for (int half = 0; half < 2; ++half) {
+            const long long step = 2 * pass + half, steps = 2 * passes;
+            q.fill_row0 = a.vocab * step / steps;
+            q.fill_rows = a.accumulate ? 0 : a.vocab * (step + 1) / steps - q.fill_row0;
+            const dim3 grid(L.tiles + q.fill_ctas);
+            if (cudaError_t e = launch_pdl(half ? embed_scatter_kernel : embed_hist_kernel, grid,
+                                           dim3(EmbedSort::THREADS), 0, s, q))
+                return e;
+        }
+    }
+    const EmbedSumParams u{a.dtable, a.dout, key[passes & 1], tok[passes & 1],
+                           reinterpret_cast<float *>(ws + L.head), reinterpret_cast<float *>(ws + L.tail), stride,
+                           a.dout_stride, int(a.n), int(a.vocab), int(a.d), L.chunk, L.chunks, a.scale,
+                           int(a.accumulate != 0)};
+    const bool wide = a.d % 8 == 0 && aligned16(a.dtable) && aligned16(a.dout) && stride * sw % 16 == 0 &&
+                      (a.n == 1 || a.dout_stride * sg % 16 == 0);
+    return by_type(a.dout_type, [&](auto tg) {
+        return by_type(a.dtable_type, [&](auto tw) {
+            using TG = typename decltype(tg)::type;
+            using TW = typename decltype(tw)::type;
+            const dim3 block(256);
+            const int cols = ceil_div(a.d, wide ? 256 : 32);
+            const dim3 sum_grid(ceil_div(L.chunks, 8), cols), join_grid(L.chunks, cols);
+            if (cudaError_t e = wide ? launch_pdl(embed_sum_kernel<TG, TW, 8>, sum_grid, block, 0, s, u)
+                                     : launch_pdl(embed_sum_kernel<TG, TW, 1>, sum_grid, block, 0, s, u))
+                return e;
+            return wide ? launch_pdl(embed_join_kernel<TW, 8>, join_grid, block, 0, s, u)
+                        : launch_pdl(embed_join_kernel<TW, 1>, join_grid, block, 0, s, u);
+        });
+    });
+}
+
+// ---------------------------------------------------------------- qkv_norm_rope
+constexpr int QKV_MAX_PARTS = 1024;  // CTAs of the gradient, one partial weight gradient each
+
+// Checks one tensor's strides (elements) and says whether whole 16-byte vectors fit it.
+static bool qkv_tensor_ok(const void *p, int64_t tok, int64_t head, unsigned n, unsigned heads, unsigned d, int size,
+                          bool written, bool *wide) {
+    if (!p || tok < 0 || head < 0) return false;
+    // Rows that are written must not overlap: in one order of the two strides each has room for the other.
+    if (written) {
+        const int64_t span = heads > 1 ? head * (heads - 1) + d : d, tspan = n > 1 ? tok * (int64_t(n) - 1) + d : d;
+        const bool by_tok = (heads < 2 || head >= d) && (n < 2 || tok >= span);
+        const bool by_head = (n < 2 || tok >= d) && (heads < 2 || head >= tspan);
+        if (!by_tok && !by_head) return false;
+    }
+    if (!aligned16(p) || (n > 1 && tok * size % 16) || (heads > 1 && head * size % 16)) *wide = false;
+    return true;
+}
+
+// f(V, G, NV) as integral constants for a row of half = d / 2 elements of T.
+template <int I>
+struct Int {
+    static constexpr int value = I;
+};
+template <typename T, typename F>
+static cudaError_t qkv_shape(int half, bool wide, F f) {
+    constexpr int V = 16 / int(sizeof(T));
+    if (!wide || half % V) return f(Int<1>{}, Int<32>{}, Int<8>{});
+    const int vecs = half / V;
+    if (vecs <= 4) return f(Int<V>{}, Int<4>{}, Int<1>{});
+    if (vecs <= 8) return f(Int<V>{}, Int<8>{}, Int<1>{});
+    if (vecs <= 16) return f(Int<V>{}, Int<16>{}, Int<1>{});
+    if (vecs <= 32) return f(Int<V>{}, Int<32>{}, Int<1>{});
+    if constexpr (sizeof(T) == 4) return f(Int<V>{}, Int<32>{}, Int<2>{});
+    return cudaErrorInvalidValue;
+}
+
+static cudaError_t qkv_common(QkvNormParams *p, bool *wide, unsigned n, const unsigned heads[3], unsigned d,
+                              unsigned type, unsigned weight_type, unsigned positions, const void *const x[3],
+                              const int64_t xs[3][2], void *const out[3], const int64_t outs[3][2],
+                              const void *const weight[2], const float *rc, const float *rs, const int *pos,
+                              float eps) {
+    const int size = type_size(type);
+    if (!size || !d || d > 512 || d % 2 || n > 0x7fffffffu || positions > 0x7fffffffu ||
+        (weight_type != EG_F32 && weight_type != type))
+        return cudaErrorInvalidValue;
+    *wide = true;
+    *p = QkvNormParams{};
+    for (int i = 0; i < 3; ++i) {
+        QkvPart &q = p->part[i];
+        if (heads[i] > 65536) return cudaErrorInvalidValue;
+        q.heads = int(heads[i]);
+        if (!heads[i] || !n) continue;
+        if (!qkv_tensor_ok(x[i], xs[i][0], xs[i][1], n, heads[i], d, size, false, wide) ||
+            !qkv_tensor_ok(out[i], outs[i][0], outs[i][1], n, heads[i], d, size, true, wide))
+            return cudaErrorInvalidValue;
+        q.x = x[i], q.out = out[i], q.w = i < 2 ? weight[i] : nullptr;
+        q.x_tok = xs[i][0], q.x_head = xs[i][1], q.out_tok = outs[i][0], q.out_head = outs[i][1];
+        if (q.w && !aligned16(q.w)) *wide = false;
+        if (i < 2) {
+            if (!rc || !rs) return cudaErrorInvalidValue;
+            if (!aligned16(rc) || !aligned16(rs)) *wide = false;
+        }
+    }
+    if (n && !pos) return cudaErrorInvalidValue;
+    p->rope_cos = rc, p->rope_sin = rs, p->pos = pos;
+    p->n = int(n), p->d = int(d), p->positions = int(positions), p->weight_f32 = weight_type == EG_F32, p->eps = eps;
+    return cudaSuccess;
+}
+static long long qkv_items(QkvNormParams *p, int hb) {
+    long long blocks = 0;
+    for (auto &q : p->part) q.blocks = ceil_div(q.heads, hb), blocks += q.blocks;
+    return blocks * p->n;
+}
+
+static cudaError_t qkv_norm_rope(const EgQkvNormRope &a, cudaStream_t s) {
+    QkvNormParams p;
+    bool wide;
+    const unsigned heads[3] = {a.q_heads, a.k_heads, a.v_heads};
+    if (cudaError_t e = qkv_common(&p, &wide, a.n, heads, a.d, a.type, a.weight_type, a.positions, a.x, a.x_stride,
+                                   a.out, a.out_stride, a.weight, a.rope_cos, a.rope_sin, a.pos, a.eps))
+        return e;
+    if (!p.n || !(a.q_heads + a.k_heads + a.v_heads)) return cudaSuccess;
+    return by_type(a.type, [&](auto t) {
+        using T = typename decltype(t)::type;
+        return qkv_shape<T>(p.d / 2, wide, [&](auto v, auto g, auto nv) {
+            constexpr int V = decltype(v)::value, G = decltype(g)::value, NV = decltype(nv)::value;
+            // Four heads a group once that still leaves every SM several warps, else one.
+            const bool four = qkv_items(&p, 4) * G >= 32ll * 16 * sm_count();
+            const long long items = qkv_items(&p, four ? 4 : 1);
+            const dim3 grid(ceil_div(items, 256 / G));
+            return four ? launch_pdl(qkv_norm_kernel<T, V, G, NV, 4>, grid, dim3(256), 0, s, p)
+                        : launch_pdl(qkv_norm_kernel<T, V, G, NV, 1>, grid, dim3(256), 0, s, p);
+        });
+    });
+}
+
+static cudaError_t qkv_norm_rope_grad(const EgQkvNormRopeGrad &a, cudaStream_t s) {
+    QkvNormParams p;
+    bool wide;
+    const unsigned heads[3] = {a.q_heads, a.k_heads, a.v_heads};
+    if (cudaError_t e = qkv_common(&p, &wide, a.n, heads, a.d, a.type, a.weight_type, a.positions, a.x, a.x_stride,
+                                   a.dx, a.dx_stride, a.weight, a.rope_cos, a.rope_sin, a.pos, a.eps))
+        return e;
+    for (int i = 0; i < 3; ++i) {
+        if (!heads[i] || !a.n) continue;
+        QkvPart &q = p.part[i];
+        if (!qkv_tensor_ok(a.dout[i], a.dout_stride[i][0], a.dout_stride[i][1], a.n, heads[i], a.d,
+                           type_size(a.type), false, &wide))
+            return cudaErrorInvalidValue;
+        q.g = a.dout[i], q.g_tok = a.dout_stride[i][0], q.g_head = a.dout_stride[i][1];
+    }
+    const bool want_dw = a.dweight[0] || a.dweight[1];
+    const bool any = p.n && (a.q_heads + a.k_heads + a.v_heads);
+    if (!any && (!want_dw || a.accumulate)) return cudaSuccess;
+    const uint64_t need = eg2_qkv_norm_rope_grad_workspace(
+        a.n, a.q_heads, a.k_heads > a.v_heads ? a.k_heads : a.v_heads, a.d);
+    if (want_dw && any && (!a.workspace || a.workspace_bytes < need || (reinterpret_cast<uintptr_t>(a.workspace) & 255)))
+        return cudaErrorInvalidValue;
+    p.dw = want_dw ? static_cast<float *>(a.workspace) : nullptr;
+    return by_type(a.type, [&](auto t) {
+        using T = typename decltype(t)::type;
+        int parts = 0;
+        if (any) {
+            const cudaError_t e = qkv_shape<T>(p.d / 2, wide, [&](auto v, auto g, auto nv) {
+                constexpr int V = decltype(v)::value, G = decltype(g)::value, NV = decltype(nv)::value;
+                constexpr int HB = 2;
+                const long long ctas = ceil_div(qkv_items(&p, HB), 256 / G);
+                const int most = 2 * sm_count() < QKV_MAX_PARTS ? 2 * sm_count() : QKV_MAX_PARTS;
+                parts = int(ctas < most ? ctas : most);
+                return launch_pdl(qkv_norm_grad_kernel<T, V, G, NV, HB>, dim3(parts), dim3(256),
+                                  size_t(256 / G) * 2 * p.d * 4, s, p);
+            });
+            if (e || !want_dw) return e;
+        }
+        const QkvDwParams w{{a.dweight[0], a.dweight[1]}, p.dw, parts, p.d, p.weight_f32, int(a.accumulate != 0)};
+        return launch_pdl(qkv_dw_kernel<T>, dim3(ceil_div(2 * p.d, 32)), dim3(256), 0, s, w);
+    });
+}
+
+}  // namespace eg2
+
+extern "C" {
+int eg2_launch_embed_rows(const EgEmbedRows *p, void *s) { return rc(embed_rows(*p, S(s))); }
+uint64_t eg2_embed_rows_grad_workspace(unsigned n, unsigned d) { return embed_grad_layout(n, d).total; }
+int eg2_launch_embed_rows_grad(const EgEmbedRowsGrad *p, void *s) { return rc(embed_rows_grad(*p, S(s))); }
+int eg2_launch_qkv_norm_rope(const EgQkvNormRope *p, void *s) { return rc(qkv_norm_rope(*p, S(s))); }
+uint64_t eg2_qkv_norm_rope_grad_workspace(unsigned n, unsigned q_heads, unsigned kv_heads, unsigned d) {
+    // A CTA, and so a partial row, holds at least one head of one token.
+    const uint64_t rows = uint64_t(n) * (uint64_t(q_heads) + 2 * uint64_t(kv_heads));
+    return (rows < QKV_MAX_PARTS ? rows : QKV_MAX_PARTS) * 2 * d * 4;
+}
+int eg2_launch_qkv_norm_rope_grad(const EgQkvNormRopeGrad *p, void *s) { return rc(qkv_norm_rope_grad(*p, S(s))); }
+}

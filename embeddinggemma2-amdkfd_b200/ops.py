@@ -131,6 +131,181 @@ def pool_l2(out, y, offsets, batch, width):
     _call("eg2_launch_pool_l2", _lib.EgPoolL2(_p(out), _p(y), _p(offsets), batch, width))
 
 
+# ---- typed operators and their gradients (fp32, fp16, bf16) ----
+# These check their tensors (ValueError before anything is enqueued) and run on
+# the current stream of their tensors' device, whichever device is current.
+_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+
+
+def _type(t, name):
+    code = _TYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{name} is {t.dtype}: expected float32, float16 or bfloat16")
+    return code
+
+
+def _check(t, name, shape, device=None, dtype=None, contiguous=False):
+    """A CUDA tensor of `shape` (None: any size) whose last dimension is contiguous."""
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name} is on {t.device}: expected {device or 'a CUDA device'}")
+    if t.dim() != len(shape) or any(s is not None and s != g for s, g in zip(shape, t.shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: expected {tuple('any' if s is None else s for s in shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}: expected {dtype}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}'s rows are not contiguous (last stride {t.stride(-1)})")
+
+
+def _check_ids(t, name, n, device):
+    import torch
+    _check(t, name, (n,), device, torch.int32, contiguous=True)
+
+
+def _workspace(workspace, need, device):
+    """The caller's workspace, or a fresh one on the current stream."""
+    import torch
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous and on {device}")
+    size = workspace.numel() * workspace.element_size()
+    if size < need:
+        raise ValueError(f"workspace has {size} bytes: {need} needed")
+    if size and workspace.data_ptr() % 256:
+        raise ValueError("workspace must be 256-byte aligned")
+    return workspace
+
+
+def _call_on(device, name, struct):
+    """_call on `device`, on that device's current stream."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return _call(name, struct)
+    with torch.cuda.device(device):
+        _call(name, struct)
+
+
+def embed_rows(out, table, ids, scale=1.0):
+    """out[t] = scale * table[ids[t]]; an id outside the table is padding (zeros).
+
+    out [n][d] and table [vocab][d] are float32, float16 or bfloat16 (each its
+    own), ids int32 [n]."""
+    dev = table.device
+    _check(table, "table", (None, None))
+    vocab, d = table.shape
+    _check(out, "out", (None, d), dev)
+    n = out.shape[0]
+    _check_ids(ids, "ids", n, dev)
+    _call_on(dev, "eg2_launch_embed_rows", _lib.EgEmbedRows(
+        _p(out), _p(table), _p(ids), out.stride(0), table.stride(0), n, vocab, d, _type(out, "out"),
+        _type(table, "table"), scale))
+
+
+def embed_rows_grad_workspace(n, d) -> int:
+    """Bytes of workspace for embed_rows_grad."""
+    return int(_lib.load().eg2_embed_rows_grad_workspace(n, d))
+
+
+def embed_rows_grad(dtable, dout, ids, scale=1.0, accumulate=False, workspace=None):
+    """dtable[v] = scale * sum of dout[t] over ids[t] = v, or added to dtable (accumulate)."""
+    dev = dtable.device
+    _check(dtable, "dtable", (None, None))
+    vocab, d = dtable.shape
+    _check(dout, "dout", (None, d), dev)
+    n = dout.shape[0]
+    _check_ids(ids, "ids", n, dev)
+    tw, tg = _type(dtable, "dtable"), _type(dout, "dout")
+    ws = _workspace(workspace, embed_rows_grad_workspace(n, d), dev)
+    _call_on(dev, "eg2_launch_embed_rows_grad", _lib.EgEmbedRowsGrad(
+        _p(dtable), _p(dout), _p(ids), _p(ws), ws.numel() * ws.element_size(), dtable.stride(0), dout.stride(0),
+        n, vocab, d, tw, tg, scale, int(accumulate)))
+
+
+def _heads(name, t, n, d, device, dtype):
+    """(pointer, strides, heads) of a [n][heads][d] tensor, or of None."""
+    if t is None:
+        return None, (0, 0), 0
+    _check(t, name, (n, None, d), device, dtype)
+    return _p(t), (t.stride(0), t.stride(1)), t.shape[1]
+
+
+def _qkv_args(x, weights, rope_cos, rope_sin, pos):
+    """The first given of queries, keys and values sets n, d, device and type."""
+    import torch
+    lead = next((t for t in x if t is not None), None)
+    if lead is None:
+        raise ValueError("queries, keys and values are all None")
+    _check(lead, "x", (None, None, None))
+    (n, _, d), dev = lead.shape, lead.device
+    code = _type(lead, "x")
+    if d % 2 or not 0 < d <= 512:
+        raise ValueError(f"head width {d}: expected an even number up to 512")
+    _check_ids(pos, "pos", n, dev)
+    wtypes = {w.dtype for w in weights if w is not None} or {torch.float32}
+    if len(wtypes) > 1 or not wtypes <= {torch.float32, lead.dtype}:
+        raise ValueError(f"weights are {wtypes}: expected one of float32 and {lead.dtype} for both")
+    for name, w in zip(("q_weight", "k_weight"), weights):
+        if w is not None:
+            _check(w, name, (d,), dev)
+    _check(rope_cos, "rope_cos", (None, d // 2), dev, torch.float32, contiguous=True)
+    _check(rope_sin, "rope_sin", tuple(rope_cos.shape), dev, torch.float32, contiguous=True)
+    wtype = 0 if wtypes == {torch.float32} else code
+    return n, d, dev, lead.dtype, code, wtype, rope_cos.shape[0]
+
+
+def qkv_norm_rope(q_out, k_out, v_out, q, k, v, q_weight, k_weight, rope_cos, rope_sin, pos, eps=1e-6):
+    """Per-head RMS norm of q, k [n][heads][d] with weights [d] and NEOX rotation by
+    row pos[t] of rope_cos, rope_sin [positions][d / 2]; v gets the norm alone.
+
+    Any of the three may be None with its output; a weight None is 1.  A position
+    outside the tables is padding (zeros).  An output may be its input."""
+    n, d, dev, dtype, code, wtype, positions = _qkv_args((q, k, v), (q_weight, k_weight), rope_cos, rope_sin, pos)
+    x = [_heads(name, t, n, d, dev, dtype) for name, t in (("q", q), ("k", k), ("v", v))]
+    out = [_heads(name, t, n, d, dev, dtype) for name, t in (("q_out", q_out), ("k_out", k_out), ("v_out", v_out))]
+    heads = [a[2] for a in x]
+    if heads != [a[2] for a in out]:
+        raise ValueError(f"outputs have {[a[2] for a in out]} heads, inputs {heads}")
+    L = _lib
+    _call_on(dev, "eg2_launch_qkv_norm_rope", L.EgQkvNormRope(
+        L.P3(*[a[0] for a in out]), L.P3(*[a[0] for a in x]), L.P2(_p(q_weight), _p(k_weight)), _p(rope_cos),
+        _p(rope_sin), _p(pos), L.Strides3(*[a[1] for a in out]), L.Strides3(*[a[1] for a in x]), n, *heads, d,
+        positions, code, wtype, eps))
+
+
+def qkv_norm_rope_grad_workspace(n, q_heads, kv_heads, d) -> int:
+    """Bytes of workspace for qkv_norm_rope_grad."""
+    return int(_lib.load().eg2_qkv_norm_rope_grad_workspace(n, q_heads, kv_heads, d))
+
+
+def qkv_norm_rope_grad(dq, dk, dv, dq_weight, dk_weight, dq_out, dk_out, dv_out, q, k, v, q_weight, k_weight,
+                       rope_cos, rope_sin, pos, eps=1e-6, accumulate=False, workspace=None):
+    """The gradient of qkv_norm_rope: dq, dk, dv from the outputs' gradients, and the
+    weights' gradients (None: not wanted), added to what they hold with accumulate."""
+    n, d, dev, dtype, code, wtype, positions = _qkv_args((q, k, v), (q_weight, k_weight), rope_cos, rope_sin, pos)
+    x = [_heads(name, t, n, d, dev, dtype) for name, t in (("q", q), ("k", k), ("v", v))]
+    dx = [_heads(name, t, n, d, dev, dtype) for name, t in (("dq", dq), ("dk", dk), ("dv", dv))]
+    g = [_heads(name, t, n, d, dev, dtype) for name, t in (("dq_out", dq_out), ("dk_out", dk_out), ("dv_out", dv_out))]
+    heads = [a[2] for a in x]
+    if heads != [a[2] for a in dx] or heads != [a[2] for a in g]:
+        raise ValueError(f"gradients have {[a[2] for a in dx]} and {[a[2] for a in g]} heads, inputs {heads}")
+    need = 0
+    for name, w, given in (("dq_weight", dq_weight, q_weight), ("dk_weight", dk_weight, k_weight)):
+        if w is not None:
+            if given is None:
+                raise ValueError(f"{name} is wanted of a weight that is None")
+            _check(w, name, (d,), dev, given.dtype)
+            need = qkv_norm_rope_grad_workspace(n, heads[0], max(heads[1:]), d)
+    ws = _workspace(workspace, need, dev)
+    L = _lib
+    _call_on(dev, "eg2_launch_qkv_norm_rope_grad", L.EgQkvNormRopeGrad(
+        L.P3(*[a[0] for a in dx]), L.P2(_p(dq_weight), _p(dk_weight)), L.P3(*[a[0] for a in g]),
+        L.P3(*[a[0] for a in x]), L.P2(_p(q_weight), _p(k_weight)), _p(rope_cos), _p(rope_sin), _p(pos), _p(ws),
+        ws.numel() * ws.element_size(), L.Strides3(*[a[1] for a in dx]), L.Strides3(*[a[1] for a in g]),
+        L.Strides3(*[a[1] for a in x]), n, *heads, d, positions, code, wtype, eps, int(accumulate)))
+
+
 def repack_q8(blocks, rows, k, codes, scales):
     rc = _lib.load().eg2_repack_q8(_p(blocks), rows, k, _p(codes), _p(scales), _stream())
     if rc:

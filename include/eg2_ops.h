@@ -113,6 +113,56 @@ typedef struct { float *g; const float *u; uint64_t n; unsigned tier; } EgGeluMu
 /* out[s] = L2(mean over the sequence's rows of y) (gemma2_fast.c:1000-1008). */
 typedef struct { float *out; const float *y; const unsigned *offsets; unsigned batch, width; } EgPoolL2;
 
+/* ---- Part 3: typed operators and their gradients --------------------------- */
+/* fp32, fp16 and bf16 operands of any width, for programs that train the text
+ * graph (or run it unquantized): each forward operator stands beside its Q8_0
+ * counterpart of part 2 and has its gradient next to it.  Types are the GGUF
+ * numbers EG_F32, EG_F16, EG_BF16; strides count elements; the elements of a
+ * row are contiguous.  Sums and statistics are in fp32 and every output is
+ * rounded once, to nearest even.  Gradients use no atomics on values: the same
+ * inputs give the same bits.  Outputs do not overlap inputs unless it says so.
+ * A workspace (256-byte aligned device memory) belongs to one call at a time. */
+enum { EG_F32 = 0, EG_F16 = 1, EG_BF16 = 30 };
+/* out[t] = scale * table[ids[t]], t < n; an id outside [0, vocab) is padding and
+ * gives a row of zeros.  Any d; whole 16-byte vectors (d a multiple of 8,
+ * 16-byte aligned rows) are the fast form. */
+typedef struct {
+    void *out; const void *table; const int *ids; int64_t out_stride, table_stride;
+    unsigned n, vocab, d, out_type, table_type; float scale;
+} EgEmbedRows;
+/* dtable[v] = scale * sum of dout[t] over ids[t] = v (tokens in ascending order),
+ * zero for an id that does not occur; with accumulate, added to what dtable
+ * holds (rows that do not occur are then not touched).  Padding's rows of dout
+ * are not read.  workspace: eg2_embed_rows_grad_workspace(n, d) bytes. */
+typedef struct {
+    void *dtable; const void *dout; const int *ids; void *workspace; uint64_t workspace_bytes;
+    int64_t dtable_stride, dout_stride;
+    unsigned n, vocab, d, dtable_type, dout_type; float scale; unsigned accumulate;
+} EgEmbedRowsGrad;
+/* For each token t < n and head: y = x / sqrt(mean(x^2) + eps) * weight, then for
+ * queries and keys the NEOX rotation of (y_i, y_{i + d/2}) by row pos[t] of the
+ * tables rope_cos, rope_sin [positions][d/2]; values have neither weight nor
+ * rotation.  Index 0, 1, 2 of an array: queries, keys, values; a stride pair is
+ * (token, head).  A head count of 0 leaves that tensor out; a null weight is 1.
+ * A position outside [0, positions) is padding: zeros.  d even, at most 512;
+ * weight_type is EG_F32 or type.  out may be x itself. */
+typedef struct {
+    void *out[3]; const void *x[3]; const void *weight[2]; const float *rope_cos, *rope_sin; const int *pos;
+    int64_t out_stride[3][2], x_stride[3][2];
+    unsigned n, q_heads, k_heads, v_heads, d, positions, type, weight_type; float eps;
+} EgQkvNormRope;
+/* Its gradient: dx from dout and the operator's inputs, and dweight (null: not
+ * wanted; weight_type) summed over tokens and heads, added to what it holds
+ * with accumulate.  Padding gives dx = 0 and adds nothing.  dx may be dout.
+ * workspace (needed for dweight): eg2_qkv_norm_rope_grad_workspace(n, q_heads,
+ * max(k_heads, v_heads), d) bytes. */
+typedef struct {
+    void *dx[3]; void *dweight[2]; const void *dout[3]; const void *x[3]; const void *weight[2];
+    const float *rope_cos, *rope_sin; const int *pos; void *workspace; uint64_t workspace_bytes;
+    int64_t dx_stride[3][2], dout_stride[3][2], x_stride[3][2];
+    unsigned n, q_heads, k_heads, v_heads, d, positions, type, weight_type; float eps; unsigned accumulate;
+} EgQkvNormRopeGrad;
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -159,6 +209,13 @@ int eg2_launch_post_add(const EgPostAdd *p, void *stream);
 int eg2_launch_gate_quant(const EgGateQuant *p, void *stream);
 int eg2_launch_gelu_mul(const EgGeluMul *p, void *stream);
 int eg2_launch_pool_l2(const EgPoolL2 *p, void *stream);
+/* Part 3. */
+int eg2_launch_embed_rows(const EgEmbedRows *p, void *stream);
+uint64_t eg2_embed_rows_grad_workspace(unsigned n, unsigned d);
+int eg2_launch_embed_rows_grad(const EgEmbedRowsGrad *p, void *stream);
+int eg2_launch_qkv_norm_rope(const EgQkvNormRope *p, void *stream);
+uint64_t eg2_qkv_norm_rope_grad_workspace(unsigned n, unsigned q_heads, unsigned kv_heads, unsigned d);
+int eg2_launch_qkv_norm_rope_grad(const EgQkvNormRopeGrad *p, void *stream);
 /* Repack GGUF Q8_0 blocks (34 B, device memory) into the SoA weight operand:
  * codes [rows][k] and fp32 scales [k/32][rows]. */
 int eg2_repack_q8(const void *blocks_dev, unsigned rows, unsigned k, int8_t *codes, float *scales, void *stream);

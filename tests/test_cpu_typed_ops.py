@@ -1,0 +1,130 @@
+"""Refusals of the typed operators (include/eg2_ops.h part 3) without a GPU: the
+C entry points return an error code for bad arguments before they launch
+anything, and the Python entry points raise for tensors that are not theirs."""
+import ctypes as C
+import importlib
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+INVALID = 1  # cudaErrorInvalidValue
+A = 4096     # stands for an aligned device address; nothing below gets as far as using it
+
+
+@pytest.fixture(scope="module")
+def L(eg2):
+    return eg2._lib
+
+
+def call(L, name, struct):
+    return getattr(L.load(), name)(C.byref(struct), None)
+
+
+def embed(L, **kw):
+    f = dict(out=A, table=A, ids=A, out_stride=16, table_stride=16, n=4, vocab=9, d=16, out_type=0, table_type=0,
+             scale=1.0)
+    f.update(kw)
+    return call(L, "eg2_launch_embed_rows", L.EgEmbedRows(**f))
+
+
+def embed_grad(L, **kw):
+    f = dict(dtable=A, dout=A, ids=A, workspace=A, workspace_bytes=1 << 30, dtable_stride=16, dout_stride=16, n=4,
+             vocab=9, d=16, dtable_type=0, dout_type=0, scale=1.0, accumulate=0)
+    f.update(kw)
+    return call(L, "eg2_launch_embed_rows_grad", L.EgEmbedRowsGrad(**f))
+
+
+@pytest.mark.parametrize("kw", [dict(out=None), dict(table=None), dict(ids=None), dict(d=0), dict(d=1 << 21),
+                                dict(n=1 << 31), dict(vocab=0xffffffff), dict(out_type=8), dict(table_type=2),
+                                dict(out_stride=15), dict(out_stride=-16), dict(table_stride=8)])
+def test_embed_rows_refuses(L, kw):
+    assert embed(L, **kw) == INVALID
+
+
+@pytest.mark.parametrize("kw", [dict(dtable=None), dict(dout=None), dict(ids=None), dict(workspace=None),
+                                dict(workspace=A + 16), dict(workspace_bytes=100), dict(d=0), dict(n=1 << 31),
+                                dict(vocab=0xffffffff), dict(dtable_type=8), dict(dout_type=2),
+                                dict(dtable_stride=15), dict(dout_stride=-1)])
+def test_embed_rows_grad_refuses(L, kw):
+    assert embed_grad(L, **kw) == INVALID
+
+
+def test_nothing_to_do_is_no_error(L):
+    assert embed(L, n=0, out=None, ids=None) == 0
+    assert embed_grad(L, vocab=0) == 0
+    assert embed_grad(L, n=0, accumulate=1) == 0
+    assert qkv(L, n=0) == 0
+    assert qkv(L, q_heads=0, k_heads=0, v_heads=0) == 0
+    assert qkv_grad(L, n=0, accumulate=1) == 0
+
+
+def qkv_fields(L, names, **kw):
+    s = [(4 * 64, 64)] * 3
+    f = {k: L.P3(A, A, A) for k in names}
+    f.update({k + "_stride": L.Strides3(*s) for k in names})
+    f.update(weight=L.P2(A, A), rope_cos=A, rope_sin=A, pos=A, n=5, q_heads=4, k_heads=2, v_heads=2, d=64,
+             positions=8, type=0, weight_type=0, eps=1e-6)
+    f.update(kw)
+    return f
+
+
+def qkv(L, **kw):
+    return call(L, "eg2_launch_qkv_norm_rope", L.EgQkvNormRope(**qkv_fields(L, ("out", "x"), **kw)))
+
+
+def qkv_grad(L, **kw):
+    f = dict(dweight=L.P2(A, A), workspace=A, workspace_bytes=1 << 30)
+    f.update(kw)
+    return call(L, "eg2_launch_qkv_norm_rope_grad",
+                L.EgQkvNormRopeGrad(**qkv_fields(L, ("dx", "dout", "x"), **f)))
+
+
+BAD_QKV = [dict(d=0), dict(d=63), dict(d=514), dict(type=8), dict(weight_type=1), dict(rope_cos=None),
+           dict(rope_sin=None), dict(pos=None), dict(n=1 << 31), dict(positions=1 << 31), dict(q_heads=70000)]
+
+
+@pytest.mark.parametrize("kw", BAD_QKV)
+def test_qkv_norm_rope_refuses(L, kw):
+    assert qkv(L, **kw) == INVALID
+    assert qkv_grad(L, **kw) == INVALID
+
+
+def test_qkv_norm_rope_refuses_pointers_and_strides(L):
+    over = L.Strides3((4 * 64, 63), (256, 64), (256, 64))   # heads overlap
+    tight = L.Strides3((255, 64), (256, 64), (256, 64))     # tokens overlap
+    back = L.Strides3((256, -64), (256, 64), (256, 64))
+    null = L.P3(A, None, A)
+    for s in (over, tight, back):
+        assert qkv(L, out_stride=s) == INVALID
+        assert qkv_grad(L, dx_stride=s) == INVALID
+    for kw in (dict(x=null), dict(x_stride=back)):
+        assert qkv(L, **kw) == INVALID
+        assert qkv_grad(L, **kw) == INVALID
+    assert qkv(L, out=null) == INVALID
+    for kw in (dict(dx=null), dict(dout=null), dict(dout_stride=back), dict(workspace=None), dict(workspace=A + 8),
+               dict(workspace_bytes=64)):
+        assert qkv_grad(L, **kw) == INVALID
+
+
+def test_workspace_sizes(L):
+    lib = L.load()
+    for n in (1, 7, 2048, 32767, 32768, 262144, 262145, 1_000_000):
+        for d in (1, 512):
+            size = lib.eg2_embed_rows_grad_workspace(n, d)
+            chunks = -(-n // (32 if n >= 32768 else 8))
+            assert size >= 16 * n + 8 * chunks * d and size % 256 == 0
+    assert lib.eg2_qkv_norm_rope_grad_workspace(1, 4, 2, 256) == 8 * 2 * 256 * 4
+    assert lib.eg2_qkv_norm_rope_grad_workspace(100000, 4, 2, 256) == 1024 * 2 * 256 * 4
+
+
+def test_python_entry_points_refuse_cpu_tensors(eg2):
+    ops = importlib.import_module("embeddinggemma2-amdkfd_b200.ops")
+    t, ids = torch.ones((4, 8)), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="expected a CUDA device"):
+        ops.embed_rows(t, t, ids)
+    with pytest.raises(ValueError, match="expected a CUDA device"):
+        ops.embed_rows_grad(t, t, ids)
+    x = torch.ones((4, 2, 8))
+    with pytest.raises(ValueError, match="expected a CUDA device"):
+        ops.qkv_norm_rope(x, None, None, x, None, None, None, None, t[:, :4], t[:, :4], ids)
