@@ -84,6 +84,9 @@ SIGNATURES = {
     "eg2_launch_qkv_norm_rope": (i32, [vp, vp]),
     "eg2_qkv_norm_rope_grad_workspace": (C.c_uint64, [u32, u32, u32, u32]),
     "eg2_launch_qkv_norm_rope_grad": (i32, [vp, vp]),
+    "eg2_launch_glu": (i32, [vp, vp]),
+    "eg2_glu_grad_workspace": (C.c_uint64, [u32, u32, u32]),
+    "eg2_launch_glu_grad": (i32, [vp, vp]),
     "eg2_repack_q8": (i32, [vp, u32, u32, vp, vp, vp]),
     "eg2_read_error": (i32, []),
     "eg2_clear_error": (None, []),
@@ -233,7 +236,21 @@ class EgQkvNormRopeGrad(C.Structure):
                 ("accumulate", u32)]
 
 
+class EgGlu(C.Structure):
+    _fields_ = [("out", P), ("x", P), ("w_gate", P), ("w_up", P), ("out_stride", i64), ("x_stride", i64),
+                ("w_gate_stride", i64), ("w_up_stride", i64), ("n", u32), ("k", u32), ("m", u32), ("type", u32),
+                ("act", u32)]
+
+
+class EgGluGrad(C.Structure):
+    _fields_ = [("dx", P), ("dw_gate", P), ("dw_up", P), ("dout", P), ("x", P), ("w_gate", P), ("w_up", P),
+                ("workspace", P), ("workspace_bytes", u64), ("dx_stride", i64), ("dw_gate_stride", i64),
+                ("dw_up_stride", i64), ("dout_stride", i64), ("x_stride", i64), ("w_gate_stride", i64),
+                ("w_up_stride", i64), ("n", u32), ("k", u32), ("m", u32), ("type", u32), ("act", u32),
+                ("dw_type", u32), ("accumulate", u32)]
+
+
 STRUCTS = {c.__name__: c for c in (EgGather, EgMM, EgNorm, EgRope, EgAttention, EgElement, EgPool, EgNormResidual,
                                    EgNormRope, EgEmbed, EgPleProj, EgNormQuant, EgQ8MM, EgQ8GeGLU, EgQkvPost, EgAttentionF16,
                                    EgPostAdd, EgGateQuant, EgGeluMul, EgPoolL2, EgEmbedRows, EgEmbedRowsGrad, EgQkvNormRope,
-                                   EgQkvNormRopeGrad)}
+                                   EgQkvNormRopeGrad, EgGlu, EgGluGrad)}

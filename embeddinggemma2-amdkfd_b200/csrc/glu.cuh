@@ -1,0 +1,463 @@
+// Gated feed-forward projection and its gradient on the 5th-generation tensor
+// cores, fp16 or bf16 operands, fp32 accumulators in tensor memory:
+//
+//   G = x Wg^T, U = x Wu^T, out = act(G) * U           (x [n][k], Wg, Wu [m][k], out [n][m])
+//
+// and, from dout = dL/dout, with G and U computed again from x:
+//
+//   dG = dout U act'(G), dU = dout act(G)              (GLU_DGRAD: rounded once to the operands' type,
+//                                                       since the next products take them as operands)
+//   dx = dG Wg + dU Wu, dWg = dG^T x, dWu = dU^T x     (GLU_PRODUCTS)
+//
+// act is gelu_tanh(g) = g s(2 c (g + 0.044715 g^3)), c = sqrt(2/pi), or silu(g) =
+// g s(g), with the logistic s(z) = 1 / (1 + exp(-z)): gelu's 0.5 (1 + tanh v) is
+// s(2 v), which keeps its relative precision where tanh is near -1.
+//
+// One kernel carries all of it.  A cluster of two CTAs (two SMs) owns one output
+// tile of 256 rows x BN columns: each CTA loads its own 128 rows of A and half of
+// B's columns, and one tcgen05.mma.cta_group::2 per 16 of K, issued by the even
+// CTA, reads both halves, so each SM fetches 32 KB per 64 of K where a tile of its
+// own (128 x 256) would fetch 48 KB: the L2-to-SM path is what such tiles run
+// into first.  The gate and up projections are one product: the even CTA's half
+// of B is the gate's weight rows, the odd one's the up projection's, and the
+// accumulator holds a gate column and its up column BN / 2 apart in the same
+// lane, where the epilogue pairs them.
+//
+// Operands arrive by TMA in boxes of 64 elements (128 bytes, 128-byte swizzle) x
+// up to 64 rows; an operand whose K runs along the rows in memory (the weights in
+// dx, everything in dW) is taken as it lies, as an MN-major operand.  What lies
+// outside a tensor is filled with zeros on both sides of a product, and what
+// lies outside the output is not stored, so n is free and k, m are multiples of 8
+// (the 16-byte row pitch of a tensor map).
+//
+// Per CTA: warp 0 TMA producer, warp 1 MMA issuer (even CTA) and owner of tensor
+// memory, warps 4..11 epilogue (lane quadrant = warp % 4, half of the columns
+// each).  Two accumulators of BN columns, so that a tile's epilogue runs under
+// the next tile's products.  Persistent: a cluster takes every (gridDim / 2)th tile.
+#pragma once
+#include "typed.cuh"
+
+namespace eg2 {
+
+enum : int { GLU_FORWARD = 0, GLU_DGRAD = 1, GLU_PRODUCTS = 2 };
+enum : int { ACT_GELU_TANH = 0, ACT_SILU = 1 };
+
+template <int BN_>
+struct GluCfg {
+    static constexpr int BN = BN_, BM = 256, BK = 64;  // one cluster's tile
+    static constexpr int STAGES = 6, THREADS = 12 * 32, EPI_WARPS = 8;
+    static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = BN / 2 * BK * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr int B_ROWS = BN / 2 < 64 ? BN / 2 : 64;  // rows of a weight box
+    static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 256;
+};
+
+struct GluMaps {
+    CUtensorMap x, wg, wu, dg, du;  // dg, du: GLU_PRODUCTS only
+};
+struct GluParams {
+    int n, k, m;
+    const void *dout;             // GLU_DGRAD
+    long long dout_stride;
+    void *out[3];                 // FORWARD: out; DGRAD: dG, dU; PRODUCTS: dx, dWg, dWu (null: not wanted)
+    long long out_stride[3];
+    int dw_f32, dw_accumulate;    // PRODUCTS: the weight gradients' type, and whether they are added to
+    int tiles, dx_tiles, group;   // tiles in all; those of dx come first; row tiles walked together
+};
+
+// ---------------------------------------------------------------- cluster pieces
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// The address, in the cluster's shared window, of the even CTA's copy of p.
+__device__ __forceinline__ uint32_t even_cta_addr(const void *p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// 2-D tiled load into this CTA's shared memory that completes on a barrier of
+// the pair; c0 is a multiple of 64 16-bit elements at every call.
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Arrives at the barrier at this offset in both CTAs once the MMAs issued so far completed.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(
+            smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// ---------------------------------------------------------------- activation
+// s(z) = 1 / (1 + 2^(-z log2 e)) from the approximate 2^x and reciprocal, each
+// within a few 2^-23 of its value: far below the operands' types.
+__device__ __forceinline__ float logistic(float z) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(-1.4426950408889634f * z)));
+    return r;
+}
+constexpr float GELU_A = 1.5957691216057308f, GELU_B = 0.071354816272600247f;  // 2 sqrt(2/pi) times 1 and 0.044715
+template <int ACT>
+__device__ __forceinline__ float glu_act(float g) {
+    return ACT == ACT_SILU ? g * logistic(g) : g * logistic(g * fmaf(GELU_B * g, g, GELU_A));
+}
+// act(g) and act'(g) = s (1 + g z' (1 - s)).
+template <int ACT>
+__device__ __forceinline__ float glu_act_grad(float g, float *act) {
+    const float g2 = g * g;
+    const float s = logistic(ACT == ACT_SILU ? g : g * fmaf(GELU_B, g2, GELU_A));
+    const float dz = ACT == ACT_SILU ? 1.0f : fmaf(3.0f * GELU_B, g2, GELU_A);
+    *act = g * s;
+    return s * fmaf(g * dz, 1.0f - s, 1.0f);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// ---------------------------------------------------------------- tiles
+// kind 0: the projections' tile or dx's; kinds 1 and 2: dWg's and dWu's.
+struct GluTile {
+    int kind, row0, col0, steps;
+};
+template <int MODE, int BN>
+__device__ __forceinline__ GluTile glu_tile(const GluParams &p, int i) {
+    const int steps_m = (p.m + 63) / 64;
+    int kind = 0, rows = p.n, cols = p.m, bn = BN / 2, steps = (p.k + 63) / 64;
+    if (MODE == GLU_PRODUCTS) {
+        cols = p.k, bn = BN, steps = 2 * steps_m;
+        if (i >= p.dx_tiles) {
+            i -= p.dx_tiles;
+            rows = p.m, steps = (p.n + 63) / 64;
+            kind = p.out[1] ? 1 : 2;
+            const int each = ((rows + 255) / 256) * ((cols + bn - 1) / bn);
+            if (i >= each) i -= each, kind = 2;
+        }
+    }
+    // `group` row tiles are walked together, column by column, so that the tiles
+    // running at one time share their operands in L2.
+    const int tm = (rows + 255) / 256, tn = (cols + bn - 1) / bn;
+    const int band = i / (p.group * tn), r0 = band * p.group, height = min(p.group, tm - r0);
+    const int j = i - band * p.group * tn;
+    return {kind, (r0 + j % height) * 256, (j / height) * bn, steps};
+}
+
+template <int MODE, int BN, typename T, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS, 1)
+    glu_kernel(const __grid_constant__ GluMaps maps, const __grid_constant__ GluParams p) {
+    using C = GluCfg<BN>;
+    static_assert(sizeof(T) == 2, "16-bit operands");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = align_smem_1024(smem_raw);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + size_t(C::STAGES) * C::STAGE);
+    uint64_t *full = bars, *empty = full + C::STAGES, *accfull = empty + C::STAGES, *accempty = accfull + 2;
+    uint64_t *mdone = accempty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mdone + 1);
+    volatile int *abort = reinterpret_cast<int *>(tmem_slot + 1);
+    auto a_tile = [&](int s) { return smem + s * C::STAGE; };
+    auto b_tile = [&](int s) { return smem + s * C::STAGE + C::A_BYTES; };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = int(cluster_rank()), cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+    if (threadIdx.x == 0) {
+        tma_prefetch(&maps.x), tma_prefetch(&maps.wg), tma_prefetch(&maps.wu);
+        *abort = 0;
+        for (int s = 0; s < C::STAGES; ++s) bar_init(&full[s], 1), bar_init(&empty[s], 1);
+        for (int b = 0; b < 2; ++b) bar_init(&accfull[b], 1), bar_init(&accempty[b], 2 * C::EPI_WARPS);
+        bar_init(mdone, 1);
+        fence_bar_init();
+    }
+    if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+    pdl_wait();
+    pdl_trigger();
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int i = cluster; ok && i < p.tiles; i += clusters) {
+                const GluTile t = glu_tile<MODE, BN>(p, i);
+                for (int kb = 0; kb < t.steps; ++kb, ++it) {
+                    const int s = it % C::STAGES;
+                    if (!wait_bar(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort)) {
+                        ok = false;
+                        break;
+                    }
+                    // The even CTA's barrier counts both CTAs' bytes.
+                    if (rank == 0) bar_expect_tx(&full[s], 2 * C::STAGE);
+                    const uint32_t bar = even_cta_addr(&full[s]);
+                    uint8_t *a = a_tile(s), *b = b_tile(s);
+                    const int arow = t.row0 + rank * 128;
+                    if (MODE != GLU_PRODUCTS) {
+                        for (int j = 0; j < 2; ++j) tma_load_2d_pair(a + j * 8192, &maps.x, bar, kb * 64, arow + j * 64);
+                        for (int j = 0; j < BN / 2 / C::B_ROWS; ++j)
+                            tma_load_2d_pair(b + j * 8192, rank ? &maps.wu : &maps.wg, bar, kb * 64, t.col0 + j * 64);
+                    } else {
+                        const int bcol = t.col0 + rank * (BN / 2);
+                        if (t.kind == 0) {
+                            const int per = t.steps / 2, seg = kb >= per, k0 = (kb - seg * per) * 64;
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_2d_pair(a + j * 8192, seg ? &maps.du : &maps.dg, bar, k0, arow + j * 64);
+                            for (int j = 0; j < BN / 128; ++j)
+                                tma_load_2d_pair(b + j * 8192, seg ? &maps.wu : &maps.wg, bar, bcol + j * 64, k0);
+                        } else {
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_2d_pair(a + j * 8192, t.kind == 1 ? &maps.dg : &maps.du, bar, arow + j * 64, kb * 64);
+                            for (int j = 0; j < BN / 128; ++j)
+                                tma_load_2d_pair(b + j * 8192, &maps.x, bar, bcol + j * 64, kb * 64);
+                        }
+                    }
+                }
+            }
+            // Drain: the MMAs have released the last loads' stages, so no arrival at
+            // this CTA's barriers is still on its way when the cluster ends; and
+            // (whatever happened) the loads themselves have landed: the even
+            // CTA's barriers cover the odd one's too.
+            const int last = it > C::STAGES ? it - C::STAGES : 0;
+            for (int j = last; ok && j < it; ++j) ok = wait_bar(&empty[j % C::STAGES], (j / C::STAGES) & 1, abort);
+            if (rank == 0)
+                for (int j = last; j < it; ++j) wait_bar(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (rank == 0 && lane == 0) {
+            constexpr uint32_t FMT = sizeof(T) == 2 && !std::is_same<T, __half>::value ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t BASE = (1u << 4) | FMT | (uint32_t(BN >> 3) << 17) | (uint32_t(C::BM >> 4) << 24);
+            int it = 0, ti = 0;
+            bool ok = true;
+            for (int i = cluster; ok && i < p.tiles; i += clusters, ++ti) {
+                const GluTile t = glu_tile<MODE, BN>(p, i);
+                const int buf = ti & 1;
+                const bool a_mn = MODE == GLU_PRODUCTS && t.kind != 0;
+                constexpr bool b_mn = MODE == GLU_PRODUCTS;
+                const uint32_t idesc = BASE | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+                if (!wait_bar(&accempty[buf], ((ti >> 1) & 1) ^ 1, abort)) break;
+                tc_fence_after();
+                for (int kb = 0; kb < t.steps; ++kb, ++it) {
+                    const int s = it % C::STAGES;
+                    if (!wait_bar(&full[s], (it / C::STAGES) & 1, abort)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(a_tile(s)), b = smem_u32(b_tile(s));
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t ad = a_mn ? desc_mn_sw128(a + kk * 2048, 8192) : desc_sw128(a + kk * 32);
+                        const uint64_t bd = b_mn ? desc_mn_sw128(b + kk * 2048, 8192) : desc_sw128(b + kk * 32);
+                        mma_f16_pair(tmem + uint32_t(buf * BN), ad, bd, idesc, kb > 0 || kk > 0 ? 1u : 0u);
+                    }
+                    tc_commit_pair(&empty[s]);
+                }
+                if (ok) tc_commit_pair(&accfull[buf]);
+            }
+            // Drain: every MMA issued above has completed before tensor memory is freed.
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                             smem_u32(mdone))
+                         : "memory");
+            wait_bar(mdone, 0, nullptr);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ epilogue
+        const int quad = warp & 3, part = (warp - 4) >> 2;
+        const uint32_t lanes = tmem + (uint32_t(quad * 32) << 16);
+        int ti = 0;
+        for (int i = cluster; i < p.tiles; i += clusters, ++ti) {
+            const GluTile t = glu_tile<MODE, BN>(p, i);
+            const int buf = ti & 1, row = t.row0 + rank * 128 + quad * 32 + lane;
+            if (!__all_sync(0xffffffffu, wait_bar(&accfull[buf], (ti >> 1) & 1, abort))) break;
+            tc_fence_after();
+            const uint32_t acc = lanes + uint32_t(buf * BN);
+            if constexpr (MODE == GLU_PRODUCTS) {
+                const bool dw = t.kind != 0;
+                const int rows = dw ? p.m : p.n;
+                for (int c0 = part * (BN / 2); c0 < (part + 1) * (BN / 2); c0 += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(acc + uint32_t(c0), r);
+                    tmem_wait_ld();
+                    reg_fence(r);
+                    const int col = t.col0 + c0;
+                    if (row < rows) {
+                        if (dw && p.dw_f32) {
+                            float *dst = static_cast<float *>(p.out[t.kind]) + row * p.out_stride[t.kind] + col;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                if (col + 4 * j >= p.k) break;
+                                float4 v = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                       __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+                                if (p.dw_accumulate) {
+                                    const float4 o = reinterpret_cast<const float4 *>(dst)[j];
+                                    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+                                }
+                                reinterpret_cast<float4 *>(dst)[j] = v;
+                            }
+                        } else {
+                            T *dst = static_cast<T *>(p.out[t.kind]) + row * p.out_stride[t.kind] + col;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (col + 8 * j >= p.k) break;
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    w[e] = pack2<T>(__uint_as_float(r[8 * j + 2 * e]),
+                                                    __uint_as_float(r[8 * j + 2 * e + 1]));
+                                reinterpret_cast<uint4 *>(dst)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                }
+            } else {
+                // Gate columns 0 .. BN/2 - 1 of the accumulator, up columns BN/2 ..; this warp's half of each.
+                constexpr int STEP = BN / 4 < 32 ? BN / 4 : 32;
+                for (int c0 = part * (BN / 4); c0 < (part + 1) * (BN / 4); c0 += STEP) {
+                    uint32_t g[STEP], u[STEP];
+                    if constexpr (STEP == 32) {
+                        tmem_ld32(acc + uint32_t(c0), g);
+                        tmem_ld32(acc + uint32_t(BN / 2 + c0), u);
+                    } else {
+                        tmem_ld16(acc + uint32_t(c0), g);
+                        tmem_ld16(acc + uint32_t(BN / 2 + c0), u);
+                    }
+                    tmem_wait_ld();
+                    reg_fence(g), reg_fence(u);
+                    const int col = t.col0 + c0;
+                    if (row >= p.n) continue;
+#pragma unroll
+                    for (int j = 0; j < STEP / 8; ++j) {
+                        if (col + 8 * j >= p.m) break;
+                        uint32_t w[4];
+                        if constexpr (MODE == GLU_FORWARD) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int z = 8 * j + 2 * e;
+                                w[e] = pack2<T>(glu_act<ACT>(__uint_as_float(g[z])) * __uint_as_float(u[z]),
+                                                glu_act<ACT>(__uint_as_float(g[z + 1])) * __uint_as_float(u[z + 1]));
+                            }
+                            T *dst = static_cast<T *>(p.out[0]) + row * p.out_stride[0] + col;
+                            reinterpret_cast<uint4 *>(dst)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                        } else {
+                            Pack<T, 8> d;
+                            d.load(static_cast<const T *>(p.dout) + row * p.dout_stride + col + 8 * j);
+                            float dh[8];
+                            d.get(dh);
+                            uint32_t v[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int z = 8 * j + 2 * e;
+                                float a0, a1;
+                                const float d0 = glu_act_grad<ACT>(__uint_as_float(g[z]), &a0);
+                                const float d1 = glu_act_grad<ACT>(__uint_as_float(g[z + 1]), &a1);
+                                w[e] = pack2<T>(dh[2 * e] * __uint_as_float(u[z]) * d0,
+                                                dh[2 * e + 1] * __uint_as_float(u[z + 1]) * d1);
+                                v[e] = pack2<T>(dh[2 * e] * a0, dh[2 * e + 1] * a1);
+                            }
+                            const long long at = row * p.out_stride[0] + col;
+                            reinterpret_cast<uint4 *>(static_cast<T *>(p.out[0]) + at)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                            reinterpret_cast<uint4 *>(static_cast<T *>(p.out[1]) + at)[j] = make_uint4(v[0], v[1], v[2], v[3]);
+                        }
+                    }
+                }
+            }
+            // The accumulator is free for the tile after next once both CTAs' warps have read it.
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(even_cta_addr(&accempty[buf]));
+        }
+    }
+    // Both CTAs' barriers and shared memory stay until neither uses the other's.
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
+    __syncwarp();
+    cluster_sync_all();
+}
+
+// A few rows (single tokens in serving): the weights' bytes are what there is to
+// move, and the tensor cores' 256-row tiles would be empty.  A warp takes one
+// output column: both weight rows stream through registers once, against up to NT rows of x.
+template <typename T, int ACT, int NT>
+__global__ void __launch_bounds__(256) glu_rows_kernel(T *__restrict__ out, long long out_stride,
+                                                       const T *__restrict__ x, long long x_stride,
+                                                       const T *__restrict__ wg, long long wg_stride,
+                                                       const T *__restrict__ wu, long long wu_stride, int n, int k, int m) {
+    pdl_wait();
+    pdl_trigger();
+    const int col = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (col >= m) return;
+    float g[NT], u[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) g[t] = u[t] = 0.0f;
+#pragma unroll 2
+    for (int c = lane * 8; c < k; c += 256) {
+        Pack<T, 8> a, b;
+        a.load(wg + col * wg_stride + c);
+        b.load(wu + col * wu_stride + c);
+        float fa[8], fb[8];
+        a.get(fa), b.get(fb);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (t >= n) break;
+            Pack<T, 8> y;
+            float fx[8];
+            y.load(x + t * x_stride + c);
+            y.get(fx);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[t] = fmaf(fx[e], fa[e], g[t]), u[t] = fmaf(fx[e], fb[e], u[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float gs = warp_sum_f(g[t]), us = warp_sum_f(u[t]);
+        if (lane == 0 && t < n) out[t * out_stride + col] = from_f32<T>(glu_act<ACT>(gs) * us);
+    }
+}
+
+}  // namespace eg2

@@ -1,0 +1,186 @@
+// Launchers and C entry points (include/eg2_ops.h, part 3) of the gated
+// feed-forward projection.  Included once, at the end of kernels.cu.
+#pragma once
+#include "glu.cuh"
+
+namespace eg2 {
+
+constexpr unsigned GLU_FEW_ROWS = 8;  // up to this many rows run on the CUDA cores
+
+// [rows][width] of a 16-bit type, boxes of 64 elements x box_rows, 128-byte swizzle.
+static bool glu_tmap(CUtensorMap *map, unsigned type, const void *base, int64_t stride, unsigned width, unsigned rows,
+                     unsigned box_rows) {
+    return encode_tmap_2d(map, type == EG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          base, width, rows, uint64_t(stride) * 2, 64, box_rows, true);
+}
+// A [rows][width] matrix of `size`-byte elements that a tensor map or 16-byte accesses can take.
+static bool glu_matrix_ok(const void *p, int64_t *stride, unsigned width, unsigned rows, int size) {
+    if (rows < 2) *stride = width;
+    return p && aligned16(p) && *stride >= int64_t(width) && *stride * size % 16 == 0 && *stride < (1ll << 36);
+}
+static int glu_tiles(unsigned rows, unsigned cols, int bn) { return ceil_div(rows, 256) * ceil_div(cols, bn); }
+
+// f(type tag, activation) for the kernels' template arguments.
+template <typename F>
+static cudaError_t glu_dispatch(unsigned type, unsigned act, F f) {
+    if (act > 1) return cudaErrorInvalidValue;
+    if (type == EG_F16) return act ? f(Tag<__half>{}, Int<1>{}) : f(Tag<__half>{}, Int<0>{});
+    if (type == EG_BF16) return act ? f(Tag<__nv_bfloat16>{}, Int<1>{}) : f(Tag<__nv_bfloat16>{}, Int<0>{});
+    return cudaErrorInvalidValue;
+}
+template <int MODE, int BN, typename T, int ACT>
+static cudaError_t glu_go(const GluMaps &maps, const GluParams &p, cudaStream_t s) {
+    static std::mutex mu;
+    static bool done[64] = {};
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    {
+        std::lock_guard<std::mutex> g(mu);
+        if (dev >= 64 || !done[dev]) {
+            if (cudaError_t e = cudaFuncSetAttribute(glu_kernel<MODE, BN, T, ACT>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     int(GluCfg<BN>::SMEM)))
+                return e;
+            if (dev < 64) done[dev] = true;
+        }
+    }
+    const int pairs = sm_count() / 2;
+    return launch_pdl(glu_kernel<MODE, BN, T, ACT>, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)),
+                      dim3(GluCfg<BN>::THREADS), GluCfg<BN>::SMEM, s, maps, p);
+}
+// The widest tile that still gives every pair of SMs one, by the time of the
+// slowest pair: a 128-column step costs about 0.6 of a 256-column one, a
+// 64-column step 0.5.
+static int glu_pick_bn(const int tiles[3]) {
+    static const int cost[3] = {50, 60, 100};
+    const int pairs = sm_count() / 2;
+    int best = 2;
+    for (int i = 1; i >= 0; --i)
+        if (tiles[i] && ceil_div(tiles[i], pairs) * cost[i] < ceil_div(tiles[best], pairs) * cost[best]) best = i;
+    return 64 << best;
+}
+
+static cudaError_t glu_check(unsigned n, unsigned k, unsigned m, unsigned type, unsigned act) {
+    if ((type != EG_F16 && type != EG_BF16) || act > 1 || !k || !m || k % 8 || m % 8 || n > 0x7fffff00u ||
+        k > (1u << 24) || m > (1u << 24))
+        return cudaErrorInvalidValue;
+    return cudaSuccess;
+}
+
+template <int MODE>
+static cudaError_t glu_project(const void *x, int64_t xs, const void *wg, int64_t wgs, const void *wu, int64_t wus,
+                               unsigned type, unsigned act, GluParams &p, cudaStream_t s) {
+    GluMaps maps{};
+    int tiles[3];
+    for (int i = 0; i < 3; ++i) tiles[i] = glu_tiles(unsigned(p.n), unsigned(p.m), 32 << i);
+    const int bn = glu_pick_bn(tiles);
+    const unsigned wrows = bn == 64 ? 32 : 64;
+    if (!glu_tmap(&maps.x, type, x, xs, unsigned(p.k), unsigned(p.n), 64) ||
+        !glu_tmap(&maps.wg, type, wg, wgs, unsigned(p.k), unsigned(p.m), wrows) ||
+        !glu_tmap(&maps.wu, type, wu, wus, unsigned(p.k), unsigned(p.m), wrows))
+        return cudaErrorInvalidValue;
+    p.tiles = glu_tiles(unsigned(p.n), unsigned(p.m), bn / 2);
+    p.group = 8;
+    return glu_dispatch(type, act, [&](auto t, auto a) {
+        using T = typename decltype(t)::type;
+        constexpr int ACT = decltype(a)::value;
+        if (bn == 256) return glu_go<MODE, 256, T, ACT>(maps, p, s);
+        if (bn == 128) return glu_go<MODE, 128, T, ACT>(maps, p, s);
+        return glu_go<MODE, 64, T, ACT>(maps, p, s);
+    });
+}
+
+static cudaError_t glu(const EgGlu &a, cudaStream_t s) {
+    if (cudaError_t e = glu_check(a.n, a.k, a.m, a.type, a.act)) return e;
+    if (!a.n) return cudaSuccess;
+    int64_t xs = a.x_stride, gs = a.w_gate_stride, us = a.w_up_stride, os = a.out_stride;
+    if (!glu_matrix_ok(a.x, &xs, a.k, a.n, 2) || !glu_matrix_ok(a.w_gate, &gs, a.k, a.m, 2) ||
+        !glu_matrix_ok(a.w_up, &us, a.k, a.m, 2) || !glu_matrix_ok(a.out, &os, a.m, a.n, 2))
+        return cudaErrorInvalidValue;
+    if (a.n <= GLU_FEW_ROWS)
+        return glu_dispatch(a.type, a.act, [&](auto t, auto act) {
+            using T = typename decltype(t)::type;
+            constexpr int ACT = decltype(act)::value;
+            const dim3 grid(ceil_div(a.m, 8));
+            auto go = [&](auto kernel) {
+                return launch_pdl(kernel, grid, dim3(256), 0, s, static_cast<T *>(a.out), (long long)os,
+                                  static_cast<const T *>(a.x), (long long)xs, static_cast<const T *>(a.w_gate),
+                                  (long long)gs, static_cast<const T *>(a.w_up), (long long)us, int(a.n), int(a.k),
+                                  int(a.m));
+            };
+            if (a.n == 1) return go(glu_rows_kernel<T, ACT, 1>);
+            if (a.n <= 4) return go(glu_rows_kernel<T, ACT, 4>);
+            return go(glu_rows_kernel<T, ACT, 8>);
+        });
+    GluParams p{};
+    p.n = int(a.n), p.k = int(a.k), p.m = int(a.m);
+    p.out[0] = a.out, p.out_stride[0] = os;
+    return glu_project<GLU_FORWARD>(a.x, xs, a.w_gate, gs, a.w_up, us, a.type, a.act, p, s);
+}
+
+static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
+    if (cudaError_t e = glu_check(a.n, a.k, a.m, a.type, a.act)) return e;
+    if ((a.dw_type != EG_F32 && a.dw_type != a.type) || (a.accumulate && a.dw_type != EG_F32))
+        return cudaErrorInvalidValue;
+    const int dws = type_size(a.dw_type);
+    int64_t xs = a.x_stride, gs = a.w_gate_stride, us = a.w_up_stride, os = a.dout_stride, dxs = a.dx_stride;
+    int64_t dgs = a.dw_gate_stride, dus = a.dw_up_stride;
+    if ((a.dw_gate && !glu_matrix_ok(a.dw_gate, &dgs, a.k, a.m, dws)) ||
+        (a.dw_up && !glu_matrix_ok(a.dw_up, &dus, a.k, a.m, dws)))
+        return cudaErrorInvalidValue;
+    if (!a.n) {  // no tokens: the weights' gradients are zero
+        if (a.accumulate) return cudaSuccess;
+        for (int i = 0; i < 2; ++i) {
+            void *w = i ? a.dw_up : a.dw_gate;
+            if (!w) continue;
+            if (cudaError_t e = cudaMemset2DAsync(w, size_t(i ? dus : dgs) * dws, 0, size_t(a.k) * dws, a.m, s))
+                return e;
+        }
+        return cudaSuccess;
+    }
+    if (!glu_matrix_ok(a.x, &xs, a.k, a.n, 2) || !glu_matrix_ok(a.w_gate, &gs, a.k, a.m, 2) ||
+        !glu_matrix_ok(a.w_up, &us, a.k, a.m, 2) || !glu_matrix_ok(a.dout, &os, a.m, a.n, 2) ||
+        (a.dx && !glu_matrix_ok(a.dx, &dxs, a.k, a.n, 2)))
+        return cudaErrorInvalidValue;
+    if (!a.dx && !a.dw_gate && !a.dw_up) return cudaSuccess;
+    if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255) ||
+        a.workspace_bytes < eg2_glu_grad_workspace(a.n, a.k, a.m))
+        return cudaErrorInvalidValue;
+    uint8_t *dg = static_cast<uint8_t *>(a.workspace), *du = dg + eg2_glu_grad_workspace(a.n, a.k, a.m) / 2;
+    GluParams p{};
+    p.n = int(a.n), p.k = int(a.k), p.m = int(a.m);
+    p.dout = a.dout, p.dout_stride = os;
+    p.out[0] = dg, p.out[1] = du, p.out_stride[0] = p.out_stride[1] = a.m;
+    if (cudaError_t e = glu_project<GLU_DGRAD>(a.x, xs, a.w_gate, gs, a.w_up, us, a.type, a.act, p, s)) return e;
+
+    GluMaps maps{};
+    if (!glu_tmap(&maps.x, a.type, a.x, xs, a.k, a.n, 64) || !glu_tmap(&maps.wg, a.type, a.w_gate, gs, a.k, a.m, 64) ||
+        !glu_tmap(&maps.wu, a.type, a.w_up, us, a.k, a.m, 64) || !glu_tmap(&maps.dg, a.type, dg, a.m, a.m, a.n, 64) ||
+        !glu_tmap(&maps.du, a.type, du, a.m, a.m, a.n, 64))
+        return cudaErrorInvalidValue;
+    p.out[0] = a.dx, p.out[1] = a.dw_gate, p.out[2] = a.dw_up;
+    p.out_stride[0] = dxs, p.out_stride[1] = dgs, p.out_stride[2] = dus;
+    p.dw_f32 = a.dw_type == EG_F32, p.dw_accumulate = a.accumulate != 0;
+    const int weights = (a.dw_gate != nullptr) + (a.dw_up != nullptr);
+    auto count = [&](int bn) { return (a.dx ? glu_tiles(a.n, a.k, bn) : 0) + weights * glu_tiles(a.m, a.k, bn); };
+    const int tiles[3] = {0, count(128), count(256)};
+    const int bn = glu_pick_bn(tiles);
+    p.dx_tiles = a.dx ? glu_tiles(a.n, a.k, bn) : 0;
+    p.tiles = count(bn);
+    p.group = 8;
+    return glu_dispatch(a.type, 0, [&](auto t, auto) {
+        using T = typename decltype(t)::type;
+        return bn == 256 ? glu_go<GLU_PRODUCTS, 256, T, 0>(maps, p, s) : glu_go<GLU_PRODUCTS, 128, T, 0>(maps, p, s);
+    });
+}
+
+}  // namespace eg2
+
+extern "C" {
+int eg2_launch_glu(const EgGlu *p, void *s) { return rc(glu(*p, S(s))); }
+uint64_t eg2_glu_grad_workspace(unsigned n, unsigned k, unsigned m) {
+    (void)k;
+    return 2 * ((uint64_t(n) * m * 2 + 255) / 256 * 256);
+}
+int eg2_launch_glu_grad(const EgGluGrad *p, void *s) { return rc(glu_grad(*p, S(s))); }
+}

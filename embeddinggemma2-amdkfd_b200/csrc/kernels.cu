@@ -522,3 +522,4 @@ void eg2_clear_error(void) { clear_device_error(); }
 }
 
 #include "rowops_abi.cuh"
+#include "glu_abi.cuh"

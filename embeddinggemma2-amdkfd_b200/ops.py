@@ -306,6 +306,69 @@ def qkv_norm_rope_grad(dq, dk, dv, dq_weight, dk_weight, dq_out, dk_out, dv_out,
         L.Strides3(*[a[1] for a in x]), n, *heads, d, positions, code, wtype, eps, int(accumulate)))
 
 
+_ACTS = {"gelu_tanh": 0, "silu": 1}
+
+
+def _glu_args(x, w_gate, w_up, act):
+    if act not in _ACTS:
+        raise ValueError(f"act {act!r}: expected one of {sorted(_ACTS)}")
+    dev = x.device
+    _check(x, "x", (None, None))
+    n, k = x.shape
+    code = _type(x, "x")
+    if code == 0:
+        raise ValueError("x is torch.float32: expected float16 or bfloat16")
+    _check(w_gate, "w_gate", (None, k), dev, x.dtype)
+    m = w_gate.shape[0]
+    _check(w_up, "w_up", (m, k), dev, x.dtype)
+    if k % 8 or m % 8 or not k or not m:
+        raise ValueError(f"k = {k}, m = {m}: expected multiples of 8")
+    return n, k, m, dev, code
+
+
+def glu(out, x, w_gate, w_up, act="gelu_tanh"):
+    """out = act(x w_gate^T) * (x w_up^T): x [n][k], weights [m][k], out [n][m], float16 or bfloat16.
+
+    act is "gelu_tanh" or "silu"; k and m are multiples of 8, rows 16-byte aligned."""
+    n, k, m, dev, code = _glu_args(x, w_gate, w_up, act)
+    _check(out, "out", (n, m), dev, x.dtype)
+    _call_on(dev, "eg2_launch_glu", _lib.EgGlu(
+        _p(out), _p(x), _p(w_gate), _p(w_up), out.stride(0), x.stride(0), w_gate.stride(0), w_up.stride(0), n, k, m,
+        code, _ACTS[act]))
+
+
+def glu_grad_workspace(n, k, m) -> int:
+    """Bytes of workspace for glu_grad."""
+    return int(_lib.load().eg2_glu_grad_workspace(n, k, m))
+
+
+def glu_grad(dx, dw_gate, dw_up, dout, x, w_gate, w_up, act="gelu_tanh", accumulate=False, workspace=None):
+    """The gradient of glu from dout [n][m] (None among dx, dw_gate, dw_up: not wanted).
+
+    The weights' gradients are of x's type or float32; with accumulate they are
+    float32 and added to.  Nothing is kept from the forward pass: the
+    projections are computed again."""
+    n, k, m, dev, code = _glu_args(x, w_gate, w_up, act)
+    _check(dout, "dout", (n, m), dev, x.dtype)
+    if dx is not None:
+        _check(dx, "dx", (n, k), dev, x.dtype)
+    dw_code = code
+    for name, w in (("dw_gate", dw_gate), ("dw_up", dw_up)):
+        if w is not None:
+            _check(w, name, (m, k), dev)
+            dw_code = _type(w, name)
+    if dw_gate is not None and dw_up is not None and dw_gate.dtype != dw_up.dtype:
+        raise ValueError(f"dw_gate is {dw_gate.dtype}, dw_up {dw_up.dtype}: expected one type")
+    if dw_code not in (0, code) or (accumulate and dw_code != 0 and not (dw_gate is None and dw_up is None)):
+        raise ValueError("weight gradients are float32 or x's type, float32 with accumulate")
+    ws = _workspace(workspace, glu_grad_workspace(n, k, m), dev)
+    st = lambda t: 0 if t is None else t.stride(0)
+    _call_on(dev, "eg2_launch_glu_grad", _lib.EgGluGrad(
+        _p(dx), _p(dw_gate), _p(dw_up), _p(dout), _p(x), _p(w_gate), _p(w_up), _p(ws), ws.numel() * ws.element_size(),
+        st(dx), st(dw_gate), st(dw_up), dout.stride(0), x.stride(0), w_gate.stride(0), w_up.stride(0), n, k, m, code,
+        _ACTS[act], dw_code, int(accumulate and dw_code == 0)))
+
+
 def repack_q8(blocks, rows, k, codes, scales):
     rc = _lib.load().eg2_repack_q8(_p(blocks), rows, k, _p(codes), _p(scales), _stream())
     if rc:

@@ -162,6 +162,27 @@ typedef struct {
     int64_t dx_stride[3][2], dout_stride[3][2], x_stride[3][2];
     unsigned n, q_heads, k_heads, v_heads, d, positions, type, weight_type; float eps; unsigned accumulate;
 } EgQkvNormRopeGrad;
+/* Gated feed-forward projection: out[t][c] = act(x[t] . w_gate[c]) * (x[t] . w_up[c]),
+ * x [n][k], weights [m][k], out [n][m], all EG_F16 or all EG_BF16 (type); both
+ * products, the activation and the product in one kernel (tcgen05, fp32
+ * accumulators).  act: EG_ACT_GELU_TANH or EG_ACT_SILU.  n is free, k and m are
+ * multiples of 8, rows are 16-byte aligned. */
+enum { EG_ACT_GELU_TANH = 0, EG_ACT_SILU = 1 };
+typedef struct {
+    void *out; const void *x, *w_gate, *w_up; int64_t out_stride, x_stride, w_gate_stride, w_up_stride;
+    unsigned n, k, m, type, act;
+} EgGlu;
+/* Its gradient from dout [n][m] and the operator's inputs; the projections are
+ * computed again, so nothing is kept from the forward pass.  dx [n][k] (type),
+ * dw_gate and dw_up [m][k] (dw_type: type or EG_F32; with accumulate, EG_F32
+ * only, added to what they hold); any of the three may be null.  The
+ * projections' gradients are rounded once to type between the two steps.
+ * workspace: eg2_glu_grad_workspace(n, k, m) bytes. */
+typedef struct {
+    void *dx, *dw_gate, *dw_up; const void *dout, *x, *w_gate, *w_up; void *workspace; uint64_t workspace_bytes;
+    int64_t dx_stride, dw_gate_stride, dw_up_stride, dout_stride, x_stride, w_gate_stride, w_up_stride;
+    unsigned n, k, m, type, act, dw_type, accumulate;
+} EgGluGrad;
 
 #ifdef __cplusplus
 extern "C" {
@@ -216,6 +237,9 @@ int eg2_launch_embed_rows_grad(const EgEmbedRowsGrad *p, void *stream);
 int eg2_launch_qkv_norm_rope(const EgQkvNormRope *p, void *stream);
 uint64_t eg2_qkv_norm_rope_grad_workspace(unsigned n, unsigned q_heads, unsigned kv_heads, unsigned d);
 int eg2_launch_qkv_norm_rope_grad(const EgQkvNormRopeGrad *p, void *stream);
+int eg2_launch_glu(const EgGlu *p, void *stream);
+uint64_t eg2_glu_grad_workspace(unsigned n, unsigned k, unsigned m);
+int eg2_launch_glu_grad(const EgGluGrad *p, void *stream);
 /* Repack GGUF Q8_0 blocks (34 B, device memory) into the SoA weight operand:
  * codes [rows][k] and fp32 scales [k/32][rows]. */
 int eg2_repack_q8(const void *blocks_dev, unsigned rows, unsigned k, int8_t *codes, float *scales, void *stream);

@@ -128,3 +128,48 @@ def test_python_entry_points_refuse_cpu_tensors(eg2):
     x = torch.ones((4, 2, 8))
     with pytest.raises(ValueError, match="expected a CUDA device"):
         ops.qkv_norm_rope(x, None, None, x, None, None, None, None, t[:, :4], t[:, :4], ids)
+
+
+def glu_fields(names, **kw):
+    f = {k: A for k in names}
+    width = {k: 128 if k in ("out", "dout") else 64 for k in names}
+    f.update({k + "_stride": width[k] for k in names})
+    f.update(n=20, k=64, m=128, type=30, act=0)
+    f.update(kw)
+    return f
+
+
+def glu(L, **kw):
+    return call(L, "eg2_launch_glu", L.EgGlu(**glu_fields(("out", "x", "w_gate", "w_up"), **kw)))
+
+
+def glu_grad(L, **kw):
+    f = dict(workspace=A, workspace_bytes=1 << 30, dw_type=30, accumulate=0)
+    f.update(kw)
+    names = ("dx", "dw_gate", "dw_up", "dout", "x", "w_gate", "w_up")
+    return call(L, "eg2_launch_glu_grad", L.EgGluGrad(**glu_fields(names, **f)))
+
+
+@pytest.mark.parametrize("kw", [dict(k=0), dict(m=0), dict(k=60), dict(m=124), dict(type=0), dict(type=8),
+                                dict(act=2), dict(n=1 << 31), dict(k=1 << 25), dict(x=None), dict(w_gate=None),
+                                dict(w_up=None), dict(x=A + 2), dict(w_up=A + 8), dict(x_stride=63),
+                                dict(x_stride=68), dict(w_gate_stride=-64), dict(w_up_stride=66)])
+def test_glu_refuses(L, kw):
+    assert glu(L, **kw) == INVALID
+    assert glu_grad(L, **kw) == INVALID
+
+
+@pytest.mark.parametrize("kw", [dict(dout=None), dict(dout_stride=120), dict(dout=A + 8), dict(dx_stride=32),
+                                dict(dx=A + 4), dict(dw_gate_stride=68), dict(dw_up=A + 2), dict(dw_type=1),
+                                dict(accumulate=1), dict(workspace=None), dict(workspace=A + 16),
+                                dict(workspace_bytes=2 * 20 * 128 * 2 - 1)])
+def test_glu_grad_refuses(L, kw):
+    assert glu_grad(L, **kw) == INVALID
+
+
+def test_glu_nothing_to_do(L):
+    assert glu(L, n=0, x=None, out=None) == 0
+    assert glu(L, out=None) == INVALID
+    assert glu_grad(L, n=0, dx=None, dw_gate=None, dw_up=None) == 0
+    assert glu_grad(L, n=0, dw_type=0, accumulate=1) == 0
+    assert glu_grad(L, dx=None, dw_gate=None, dw_up=None) == 0
