@@ -141,19 +141,6 @@ __device__ __forceinline__ float glu_act_grad(float g, float *act) {
     *act = g * s;
     return s * fmaf(g * dz, 1.0f - s, 1.0f);
 }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // ---------------------------------------------------------------- tiles
 // kind 0: the projections' tile or dx's; kinds 1 and 2: dWg's and dWu's.
 struct GluTile {

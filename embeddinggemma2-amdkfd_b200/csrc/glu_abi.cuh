@@ -30,20 +30,8 @@ static cudaError_t glu_dispatch(unsigned type, unsigned act, F f) {
 }
 template <int MODE, int BN, typename T, int ACT>
 static cudaError_t glu_go(const GluMaps &maps, const GluParams &p, cudaStream_t s) {
-    static std::mutex mu;
-    static bool done[64] = {};
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) return e;
-    {
-        std::lock_guard<std::mutex> g(mu);
-        if (dev >= 64 || !done[dev]) {
-            if (cudaError_t e = cudaFuncSetAttribute(glu_kernel<MODE, BN, T, ACT>,
-                                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                     int(GluCfg<BN>::SMEM)))
-                return e;
-            if (dev < 64) done[dev] = true;
-        }
-    }
+    static AllowSmem allow;
+    if (cudaError_t e = allow(glu_kernel<MODE, BN, T, ACT>, int(GluCfg<BN>::SMEM))) return e;
     const int pairs = sm_count() / 2;
     return launch_pdl(glu_kernel<MODE, BN, T, ACT>, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)),
                       dim3(GluCfg<BN>::THREADS), GluCfg<BN>::SMEM, s, maps, p);

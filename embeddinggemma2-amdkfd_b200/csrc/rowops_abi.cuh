@@ -26,6 +26,22 @@ static cudaError_t by_type(unsigned t, F f) {
     }
 }
 
+// Opts one kernel into its dynamic shared memory, once per device.
+struct AllowSmem {
+    std::mutex mu;
+    bool done[64] = {};
+    template <typename K>
+    cudaError_t operator()(K kernel, int bytes) {
+        int dev = 0;
+        if (cudaError_t e = cudaGetDevice(&dev)) return e;
+        std::lock_guard<std::mutex> g(mu);
+        if (dev < 64 && done[dev]) return cudaSuccess;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (!e && dev < 64) done[dev] = true;
+        return e;
+    }
+};
+
 // ---------------------------------------------------------------- embed_rows
 static cudaError_t embed_rows(const EgEmbedRows &a, cudaStream_t s) {
     const int so = type_size(a.out_type), st = type_size(a.table_type);
@@ -152,7 +168,7 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------- qkv_norm_rope
-constexpr int QKV_MAX_PARTS = 1024;  // CTAs of the gradient, one partial weight gradient each
+constexpr int QKV_MAX_PARTS = 1024;  // at least the gradient's CTAs (two per SM), one partial row each
 
 // Checks one tensor's strides (elements) and says whether whole 16-byte vectors fit it.
 static bool qkv_tensor_ok(const void *p, int64_t tok, int64_t head, unsigned n, unsigned heads, unsigned d, int size,
@@ -193,7 +209,7 @@ static cudaError_t qkv_common(QkvNormParams *p, bool *wide, unsigned n, const un
                               const void *const weight[2], const float *rc, const float *rs, const int *pos,
                               float eps) {
     const int size = type_size(type);
-    if (!size || !d || d > 512 || d % 2 || n > 0x7fffffffu || positions > 0x7fffffffu ||
+    if (!size || !d || d > 512 || d % 2 || n > (1u << 30) || positions > 0x7fffffffu ||
         (weight_type != EG_F32 && weight_type != type))
         return cudaErrorInvalidValue;
     *wide = true;
@@ -219,10 +235,43 @@ static cudaError_t qkv_common(QkvNormParams *p, bool *wide, unsigned n, const un
     p->n = int(n), p->d = int(d), p->positions = int(positions), p->weight_f32 = weight_type == EG_F32, p->eps = eps;
     return cudaSuccess;
 }
-static long long qkv_items(QkvNormParams *p, int hb) {
-    long long blocks = 0;
-    for (auto &q : p->part) q.blocks = ceil_div(q.heads, hb), blocks += q.blocks;
-    return blocks * p->n;
+// Shares a grid of at most `most` CTAs, each taking `per` items at a time, out
+// among the kinds by their work: an item's rows, and about half a row for the item itself.
+static int qkv_share(QkvNormParams *p, int hb, int per, int most) {
+    long long work[3], total = 0;
+    int need[3], cta[3], want = 0, big = 0;
+    for (int i = 0; i < 3; ++i) {
+        QkvPart &q = p->part[i];
+        q.blocks = ceil_div(q.heads, hb);
+        work[i] = 2 * q.heads + q.blocks;
+        total += work[i];
+        need[i] = q.heads ? ceil_div((long long)p->n * q.blocks, per) : 0;
+        if (work[i] > work[big]) big = i;
+    }
+    for (int i = 0; i < 3; ++i) {
+        const long long share = work[i] * most / total;
+        cta[i] = int(share < need[i] ? share : need[i]);
+        if (!cta[i] && need[i]) cta[i] = 1;
+        want += cta[i];
+    }
+    const int left = need[big] - cta[big] < most - want ? need[big] - cta[big] : most - want;
+    if (left > 0) cta[big] += left;
+    for (int i = 0, end = 0; i < 3; ++i) p->cta_end[i] = end += cta[i];
+    return p->cta_end[2];
+}
+template <typename T, int G, int NV, bool GRAD>
+static cudaError_t qkv_stream(QkvNormParams &p, cudaStream_t s) {
+    constexpr int V = 16 / int(sizeof(T)), HB = 2 / NV;
+    const int ctas = qkv_share(&p, HB, 256 / G, 2 * sm_count());
+    constexpr size_t smem = GRAD ? 2 * 8 * 256 * 16 : 0;  // two stages of 8 vectors per thread
+    const auto go = [&](auto kernel, AllowSmem &allow) -> cudaError_t {
+        if (GRAD)
+            if (cudaError_t e = allow(kernel, int(smem))) return e;
+        return launch_pdl(kernel, dim3(ctas), dim3(256), smem, s, p);
+    };
+    static AllowSmem exact, other;
+    return p.d / 2 == G * NV * V ? go(qkv_stream_kernel<T, G, NV, HB, GRAD, true>, exact)
+                                 : go(qkv_stream_kernel<T, G, NV, HB, GRAD, false>, other);
 }
 
 static cudaError_t qkv_norm_rope(const EgQkvNormRope &a, cudaStream_t s) {
@@ -232,17 +281,16 @@ static cudaError_t qkv_norm_rope(const EgQkvNormRope &a, cudaStream_t s) {
     if (cudaError_t e = qkv_common(&p, &wide, a.n, heads, a.d, a.type, a.weight_type, a.positions, a.x, a.x_stride,
                                    a.out, a.out_stride, a.weight, a.rope_cos, a.rope_sin, a.pos, a.eps))
         return e;
-    if (!p.n || !(a.q_heads + a.k_heads + a.v_heads)) return cudaSuccess;
+    const long long rows = (long long)p.n * (p.part[0].heads + p.part[1].heads + p.part[2].heads);
+    if (!rows) return cudaSuccess;
     return by_type(a.type, [&](auto t) {
         using T = typename decltype(t)::type;
         return qkv_shape<T>(p.d / 2, wide, [&](auto v, auto g, auto nv) {
             constexpr int V = decltype(v)::value, G = decltype(g)::value, NV = decltype(nv)::value;
-            // Four heads a group once that still leaves every SM several warps, else one.
-            const bool four = qkv_items(&p, 4) * G >= 32ll * 16 * sm_count();
-            const long long items = qkv_items(&p, four ? 4 : 1);
-            const dim3 grid(ceil_div(items, 256 / G));
-            return four ? launch_pdl(qkv_norm_kernel<T, V, G, NV, 4>, grid, dim3(256), 0, s, p)
-                        : launch_pdl(qkv_norm_kernel<T, V, G, NV, 1>, grid, dim3(256), 0, s, p);
+            // Rows enough to go round the streaming form's grid more than once, else direct.
+            if constexpr (V > 1)
+                if (rows * G > 2ll * sm_count() * 256 * 4) return qkv_stream<T, G, NV, false>(p, s);
+            return launch_pdl(qkv_norm_kernel<T, V, G, NV>, dim3(ceil_div(rows, 256 / G)), dim3(256), 0, s, p);
         });
     });
 }
@@ -272,21 +320,18 @@ static cudaError_t qkv_norm_rope_grad(const EgQkvNormRopeGrad &a, cudaStream_t s
     p.dw = want_dw ? static_cast<float *>(a.workspace) : nullptr;
     return by_type(a.type, [&](auto t) {
         using T = typename decltype(t)::type;
-        int parts = 0;
         if (any) {
             const cudaError_t e = qkv_shape<T>(p.d / 2, wide, [&](auto v, auto g, auto nv) {
                 constexpr int V = decltype(v)::value, G = decltype(g)::value, NV = decltype(nv)::value;
-                constexpr int HB = 2;
-                const long long ctas = ceil_div(qkv_items(&p, HB), 256 / G);
-                const int most = 2 * sm_count() < QKV_MAX_PARTS ? 2 * sm_count() : QKV_MAX_PARTS;
-                parts = int(ctas < most ? ctas : most);
-                return launch_pdl(qkv_norm_grad_kernel<T, V, G, NV, HB>, dim3(parts), dim3(256),
-                                  size_t(256 / G) * 2 * p.d * 4, s, p);
+                if constexpr (V > 1) return qkv_stream<T, G, NV, true>(p, s);
+                const int ctas = qkv_share(&p, 1, 8, 2 * sm_count());
+                return launch_pdl(qkv_norm_grad_kernel<T>, dim3(ctas), dim3(256), 0, s, p);
             });
             if (e || !want_dw) return e;
         }
-        const QkvDwParams w{{a.dweight[0], a.dweight[1]}, p.dw, parts, p.d, p.weight_f32, int(a.accumulate != 0)};
-        return launch_pdl(qkv_dw_kernel<T>, dim3(ceil_div(2 * p.d, 32)), dim3(256), 0, s, w);
+        const QkvDwParams w{{a.dweight[0], a.dweight[1]}, p.dw, {p.cta_end[0], p.cta_end[1]}, p.d, p.weight_f32,
+                            int(a.accumulate != 0)};
+        return launch_pdl(qkv_dw_kernel<T>, dim3(ceil_div(p.d, 32), 2), dim3(1024), 0, s, w);
     });
 }
 
@@ -300,7 +345,7 @@ int eg2_launch_qkv_norm_rope(const EgQkvNormRope *p, void *s) { return rc(qkv_no
 uint64_t eg2_qkv_norm_rope_grad_workspace(unsigned n, unsigned q_heads, unsigned kv_heads, unsigned d) {
     // A CTA, and so a partial row, holds at least one head of one token.
     const uint64_t rows = uint64_t(n) * (uint64_t(q_heads) + 2 * uint64_t(kv_heads));
-    return (rows < QKV_MAX_PARTS ? rows : QKV_MAX_PARTS) * 2 * d * 4;
+    return (rows < QKV_MAX_PARTS ? rows : QKV_MAX_PARTS) * d * 4;
 }
 int eg2_launch_qkv_norm_rope_grad(const EgQkvNormRopeGrad *p, void *s) { return rc(qkv_norm_rope_grad(*p, S(s))); }
 }

@@ -59,4 +59,77 @@ struct Pack {
     }
 };
 
+// ---------------------------------------------------------------- pairs
+// Two fp32 operations in one instruction (FFMA2 and its kin), each rounded as
+// its scalar form: half the issue slots of a row kernel's arithmetic.
+__device__ __forceinline__ uint64_t bits2(float2 a) {
+    return uint64_t(__float_as_uint(a.x)) | uint64_t(__float_as_uint(a.y)) << 32;
+}
+__device__ __forceinline__ float2 pair2(uint64_t b) {
+    return make_float2(__uint_as_float(uint32_t(b)), __uint_as_float(uint32_t(b >> 32)));
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+    return pair2(d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return pair2(d);
+}
+// A 16-byte vector of T as pairs, and back (each element rounded once).
+__device__ __forceinline__ void unpack2(const uint4 &w, float2 (&f)[2], float) {
+    f[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+    f[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+}
+__device__ __forceinline__ void unpack2(const uint4 &w, float2 (&f)[4], __half) {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __half22float2(h[i]);
+}
+__device__ __forceinline__ void unpack2(const uint4 &w, float2 (&f)[4], __nv_bfloat16) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint4 packed(const float2 (&f)[2], float) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+}
+template <typename T>
+__device__ __forceinline__ uint4 packed(const float2 (&f)[4], T) {
+    return make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y), pack2<T>(f[2].x, f[2].y),
+                      pack2<T>(f[3].x, f[3].y));
+}
+
+// ---------------------------------------------------------------- copies to shared memory
+// 16 bytes from global to shared memory, or 16 zero bytes (nothing is read) when
+// `on` is false; complete after copies_wait<K>() leaves at most K committed
+// groups of this thread outstanding.
+__device__ __forceinline__ void copy16(uint4 *dst, const void *src, bool on) {
+    asm volatile(
+        "{\n\t.reg .pred off;\n\t"
+        "setp.eq.u32 off, %2, 0;\n\t"
+        "cp.async.cg.shared.global [%0], [%1], 16, off;\n\t}" ::"r"(smem_u32(dst)),
+        "l"(src), "r"(uint32_t(on))
+        : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory");
+}
+
 }  // namespace eg2

@@ -7,6 +7,9 @@ only the allocator and stream provider here.
 from __future__ import annotations
 
 import ctypes as C
+import struct
+
+import torch
 
 from . import _lib
 
@@ -16,13 +19,12 @@ def _p(t):
 
 
 def _stream():
-    import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _call(name, struct, *extra):
+def _call(name, params, *extra):
     fn = getattr(_lib.load(), name)
-    rc = fn(C.byref(struct), *extra, _stream())
+    rc = fn(C.byref(params), *extra, _stream())
     if rc:
         raise RuntimeError(f"{name} failed with CUDA error {rc}")
 
@@ -133,58 +135,102 @@ def pool_l2(out, y, offsets, batch, width):
 
 # ---- typed operators and their gradients (fp32, fp16, bf16) ----
 # These check their tensors (ValueError before anything is enqueued) and run on
-# the current stream of their tensors' device, whichever device is current.
-_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}
+# the current stream of their tensors' device, whichever device is current.  A
+# call of a small operator is mostly host time, so a check that passes is a few
+# comparisons, and the parameters are packed straight into the C struct's bytes.
+class _Typed:
+    """One C entry point; arrays of its parameter struct are passed flat."""
+
+    CODES = {C.c_void_p: "P", C.c_int64: "q", C.c_uint64: "Q", C.c_uint: "I", C.c_float: "f"}
+
+    def __init__(self, name, cls):
+        self.name, self.fn = name, None
+        fmt = "@"
+        for _, t in cls._fields_:
+            count = 1
+            while hasattr(t, "_length_"):
+                count, t = count * t._length_, t._type_
+            fmt += f"{count}{self.CODES[t]}"
+        self.pack = struct.Struct(fmt + "0P").pack  # 0P: the struct's trailing alignment
+
+    def __call__(self, device, *values):
+        if self.fn is None:
+            self.fn = getattr(_lib.load(), self.name)
+        params, index = self.pack(*values), device.index
+        if index == torch._C._cuda_getDevice():
+            rc = self.fn(params, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = self.fn(params, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            raise RuntimeError(f"{self.name} failed with CUDA error {rc}")
+
+
+_embed_rows = _Typed("eg2_launch_embed_rows", _lib.EgEmbedRows)
+_embed_rows_grad = _Typed("eg2_launch_embed_rows_grad", _lib.EgEmbedRowsGrad)
+_qkv_norm_rope = _Typed("eg2_launch_qkv_norm_rope", _lib.EgQkvNormRope)
+_qkv_norm_rope_grad = _Typed("eg2_launch_qkv_norm_rope_grad", _lib.EgQkvNormRopeGrad)
+_glu = _Typed("eg2_launch_glu", _lib.EgGlu)
+_glu_grad = _Typed("eg2_launch_glu_grad", _lib.EgGluGrad)
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_ACTS = {"gelu_tanh": 0, "silu": 1}
 
 
 def _type(t, name):
-    code = _TYPES.get(str(t.dtype))
+    code = _TYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{name} is {t.dtype}: expected float32, float16 or bfloat16")
     return code
 
 
-def _check(t, name, shape, device=None, dtype=None, contiguous=False):
-    """A CUDA tensor of `shape` (None: any size) whose last dimension is contiguous."""
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{name} is on {t.device}: expected {device or 'a CUDA device'}")
-    if t.dim() != len(shape) or any(s is not None and s != g for s, g in zip(shape, t.shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}: expected {tuple('any' if s is None else s for s in shape)}")
-    if dtype is not None and t.dtype != dtype:
+def _lead(t, name, dims):
+    """Shape, device and strides of the tensor that sets the call's sizes."""
+    shape, stride = t.shape, t.stride()
+    if not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}: expected a CUDA device")
+    if len(shape) != dims:
+        raise ValueError(f"{name} has shape {tuple(shape)}: expected {dims} dimensions")
+    if stride[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}'s rows are not contiguous (last stride {stride[-1]})")
+    return shape, t.device, stride
+
+
+def _check(t, name, shape, device, dtype):
+    """The strides of a tensor of that shape, device and type whose last dimension is contiguous."""
+    stride = t.stride()
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: expected {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}: expected {device}")
+    if t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}: expected {dtype}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name} is not contiguous")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}'s rows are not contiguous (last stride {t.stride(-1)})")
+    if stride[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}'s rows are not contiguous (last stride {stride[-1]})")
+    return stride
 
 
-def _check_ids(t, name, n, device):
-    import torch
-    _check(t, name, (n,), device, torch.int32, contiguous=True)
+def _rows(t, name, width, device):
+    """Rows and row stride of a tensor of shape [any][width]."""
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width:
+        raise ValueError(f"{name} has shape {tuple(shape)}: expected (any, {width})")
+    return shape[0], _check(t, name, shape, device, t.dtype)[0]
 
 
 def _workspace(workspace, need, device):
-    """The caller's workspace, or a fresh one on the current stream."""
-    import torch
+    """(address, bytes, tensor) of the caller's workspace, or of a fresh one on the current stream."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
+        with torch.cuda.device(device):
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        return workspace.data_ptr(), need, workspace
+    size, ptr = workspace.numel() * workspace.element_size(), workspace.data_ptr()
     if workspace.device != device or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous and on {device}")
-    size = workspace.numel() * workspace.element_size()
     if size < need:
         raise ValueError(f"workspace has {size} bytes: {need} needed")
-    if size and workspace.data_ptr() % 256:
+    if need and ptr % 256:
         raise ValueError("workspace must be 256-byte aligned")
-    return workspace
-
-
-def _call_on(device, name, struct):
-    """_call on `device`, on that device's current stream."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        return _call(name, struct)
-    with torch.cuda.device(device):
-        _call(name, struct)
+    return ptr, size, workspace
 
 
 def embed_rows(out, table, ids, scale=1.0):
@@ -192,15 +238,11 @@ def embed_rows(out, table, ids, scale=1.0):
 
     out [n][d] and table [vocab][d] are float32, float16 or bfloat16 (each its
     own), ids int32 [n]."""
-    dev = table.device
-    _check(table, "table", (None, None))
-    vocab, d = table.shape
-    _check(out, "out", (None, d), dev)
-    n = out.shape[0]
-    _check_ids(ids, "ids", n, dev)
-    _call_on(dev, "eg2_launch_embed_rows", _lib.EgEmbedRows(
-        _p(out), _p(table), _p(ids), out.stride(0), table.stride(0), n, vocab, d, _type(out, "out"),
-        _type(table, "table"), scale))
+    (vocab, d), dev, stride = _lead(table, "table", 2)
+    n, out_stride = _rows(out, "out", d, dev)
+    _check(ids, "ids", (n,), dev, torch.int32)
+    _embed_rows(dev, out.data_ptr(), table.data_ptr(), ids.data_ptr(), out_stride, stride[0], n, vocab, d,
+                _type(out, "out"), _type(table, "table"), scale)
 
 
 def embed_rows_grad_workspace(n, d) -> int:
@@ -209,50 +251,65 @@ def embed_rows_grad_workspace(n, d) -> int:
 
 
 def embed_rows_grad(dtable, dout, ids, scale=1.0, accumulate=False, workspace=None):
-    """dtable[v] = scale * sum of dout[t] over ids[t] = v, or added to dtable (accumulate)."""
-    dev = dtable.device
-    _check(dtable, "dtable", (None, None))
-    vocab, d = dtable.shape
-    _check(dout, "dout", (None, d), dev)
-    n = dout.shape[0]
-    _check_ids(ids, "ids", n, dev)
-    tw, tg = _type(dtable, "dtable"), _type(dout, "dout")
+    """dtable[v] = scale * sum of dout[t] over ids[t] = v, or added to dtable (accumulate).
+
+    dtable [vocab][d] and dout [n][d] are float32, float16 or bfloat16 (each its
+    own), ids int32 [n]; the sums are in fp32, in token order."""
+    (vocab, d), dev, stride = _lead(dtable, "dtable", 2)
+    n, dout_stride = _rows(dout, "dout", d, dev)
+    _check(ids, "ids", (n,), dev, torch.int32)
+    types = _type(dtable, "dtable"), _type(dout, "dout")
     ws = _workspace(workspace, embed_rows_grad_workspace(n, d), dev)
-    _call_on(dev, "eg2_launch_embed_rows_grad", _lib.EgEmbedRowsGrad(
-        _p(dtable), _p(dout), _p(ids), _p(ws), ws.numel() * ws.element_size(), dtable.stride(0), dout.stride(0),
-        n, vocab, d, tw, tg, scale, int(accumulate)))
+    _embed_rows_grad(dev, dtable.data_ptr(), dout.data_ptr(), ids.data_ptr(), ws[0], ws[1], stride[0],
+                     dout_stride, n, vocab, d, *types, scale, bool(accumulate))
 
 
-def _heads(name, t, n, d, device, dtype):
-    """(pointer, strides, heads) of a [n][heads][d] tensor, or of None."""
-    if t is None:
-        return None, (0, 0), 0
-    _check(t, name, (n, None, d), device, dtype)
-    return _p(t), (t.stride(0), t.stride(1)), t.shape[1]
-
-
-def _qkv_args(x, weights, rope_cos, rope_sin, pos):
-    """The first given of queries, keys and values sets n, d, device and type."""
-    import torch
-    lead = next((t for t in x if t is not None), None)
+def _qkv_args(x, q_weight, k_weight, rope_cos, rope_sin, pos):
+    """Sizes and types; the first given of queries, keys and values sets n, d, device and type."""
+    lead = x[0] if x[0] is not None else x[1] if x[1] is not None else x[2]
     if lead is None:
         raise ValueError("queries, keys and values are all None")
-    _check(lead, "x", (None, None, None))
-    (n, _, d), dev = lead.shape, lead.device
-    code = _type(lead, "x")
+    (n, _, d), dev, _ = _lead(lead, "x", 3)
+    dtype = lead.dtype
+    code = wtype = _type(lead, "x")
     if d % 2 or not 0 < d <= 512:
         raise ValueError(f"head width {d}: expected an even number up to 512")
-    _check_ids(pos, "pos", n, dev)
-    wtypes = {w.dtype for w in weights if w is not None} or {torch.float32}
-    if len(wtypes) > 1 or not wtypes <= {torch.float32, lead.dtype}:
-        raise ValueError(f"weights are {wtypes}: expected one of float32 and {lead.dtype} for both")
-    for name, w in zip(("q_weight", "k_weight"), weights):
-        if w is not None:
-            _check(w, name, (d,), dev)
-    _check(rope_cos, "rope_cos", (None, d // 2), dev, torch.float32, contiguous=True)
-    _check(rope_sin, "rope_sin", tuple(rope_cos.shape), dev, torch.float32, contiguous=True)
-    wtype = 0 if wtypes == {torch.float32} else code
-    return n, d, dev, lead.dtype, code, wtype, rope_cos.shape[0]
+    _check(pos, "pos", (n,), dev, torch.int32)
+    wdtype = q_weight.dtype if q_weight is not None else k_weight.dtype if k_weight is not None else dtype
+    if wdtype == torch.float32:
+        wtype = 0
+    elif wdtype != dtype:
+        raise ValueError(f"weights are {wdtype}: expected float32 or {dtype}")
+    if q_weight is not None:
+        _check(q_weight, "q_weight", (d,), dev, wdtype)
+    if k_weight is not None:
+        _check(k_weight, "k_weight", (d,), dev, wdtype)
+    positions, cos_stride = _rows(rope_cos, "rope_cos", d // 2, dev)
+    sin_stride = _check(rope_sin, "rope_sin", rope_cos.shape, dev, torch.float32)[0]
+    if rope_cos.dtype != torch.float32 or (positions > 1 and not cos_stride == sin_stride == d // 2):
+        raise ValueError("rope_cos and rope_sin must be contiguous float32")
+    heads = [0 if t is None else t.shape[1] if t.dim() == 3 else -1 for t in x]
+    return (n, *heads, d, positions, code, wtype), dev, dtype
+
+
+def _qkv_tensors(names, tensors, sizes, dev, dtype):
+    """Addresses and (token, head) strides of three [n][heads][d] tensors."""
+    n, d, ptrs, strides = sizes[0], sizes[4], [], []
+    for i in (0, 1, 2):
+        t, heads = tensors[i], sizes[i + 1]
+        if t is None:
+            if heads:
+                raise ValueError(f"{names[i]} is None: expected {heads} heads")
+            ptrs.append(0)
+            strides += (0, 0)
+        else:
+            strides += _check(t, names[i], (n, heads, d), dev, dtype)[:2]
+            ptrs.append(t.data_ptr())
+    return ptrs, strides
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def qkv_norm_rope(q_out, k_out, v_out, q, k, v, q_weight, k_weight, rope_cos, rope_sin, pos, eps=1e-6):
@@ -261,17 +318,11 @@ def qkv_norm_rope(q_out, k_out, v_out, q, k, v, q_weight, k_weight, rope_cos, ro
 
     Any of the three may be None with its output; a weight None is 1.  A position
     outside the tables is padding (zeros).  An output may be its input."""
-    n, d, dev, dtype, code, wtype, positions = _qkv_args((q, k, v), (q_weight, k_weight), rope_cos, rope_sin, pos)
-    x = [_heads(name, t, n, d, dev, dtype) for name, t in (("q", q), ("k", k), ("v", v))]
-    out = [_heads(name, t, n, d, dev, dtype) for name, t in (("q_out", q_out), ("k_out", k_out), ("v_out", v_out))]
-    heads = [a[2] for a in x]
-    if heads != [a[2] for a in out]:
-        raise ValueError(f"outputs have {[a[2] for a in out]} heads, inputs {heads}")
-    L = _lib
-    _call_on(dev, "eg2_launch_qkv_norm_rope", L.EgQkvNormRope(
-        L.P3(*[a[0] for a in out]), L.P3(*[a[0] for a in x]), L.P2(_p(q_weight), _p(k_weight)), _p(rope_cos),
-        _p(rope_sin), _p(pos), L.Strides3(*[a[1] for a in out]), L.Strides3(*[a[1] for a in x]), n, *heads, d,
-        positions, code, wtype, eps))
+    sizes, dev, dtype = _qkv_args((q, k, v), q_weight, k_weight, rope_cos, rope_sin, pos)
+    x, xs = _qkv_tensors(("q", "k", "v"), (q, k, v), sizes, dev, dtype)
+    out, outs = _qkv_tensors(("q_out", "k_out", "v_out"), (q_out, k_out, v_out), sizes, dev, dtype)
+    _qkv_norm_rope(dev, *out, *x, _ptr(q_weight), _ptr(k_weight), rope_cos.data_ptr(), rope_sin.data_ptr(),
+                   pos.data_ptr(), *outs, *xs, *sizes, eps)
 
 
 def qkv_norm_rope_grad_workspace(n, q_heads, kv_heads, d) -> int:
@@ -283,58 +334,48 @@ def qkv_norm_rope_grad(dq, dk, dv, dq_weight, dk_weight, dq_out, dk_out, dv_out,
                        rope_cos, rope_sin, pos, eps=1e-6, accumulate=False, workspace=None):
     """The gradient of qkv_norm_rope: dq, dk, dv from the outputs' gradients, and the
     weights' gradients (None: not wanted), added to what they hold with accumulate."""
-    n, d, dev, dtype, code, wtype, positions = _qkv_args((q, k, v), (q_weight, k_weight), rope_cos, rope_sin, pos)
-    x = [_heads(name, t, n, d, dev, dtype) for name, t in (("q", q), ("k", k), ("v", v))]
-    dx = [_heads(name, t, n, d, dev, dtype) for name, t in (("dq", dq), ("dk", dk), ("dv", dv))]
-    g = [_heads(name, t, n, d, dev, dtype) for name, t in (("dq_out", dq_out), ("dk_out", dk_out), ("dv_out", dv_out))]
-    heads = [a[2] for a in x]
-    if heads != [a[2] for a in dx] or heads != [a[2] for a in g]:
-        raise ValueError(f"gradients have {[a[2] for a in dx]} and {[a[2] for a in g]} heads, inputs {heads}")
+    sizes, dev, dtype = _qkv_args((q, k, v), q_weight, k_weight, rope_cos, rope_sin, pos)
+    x, xs = _qkv_tensors(("q", "k", "v"), (q, k, v), sizes, dev, dtype)
+    dx, dxs = _qkv_tensors(("dq", "dk", "dv"), (dq, dk, dv), sizes, dev, dtype)
+    g, gs = _qkv_tensors(("dq_out", "dk_out", "dv_out"), (dq_out, dk_out, dv_out), sizes, dev, dtype)
+    n, hq, hk, hv, d = sizes[:5]
     need = 0
     for name, w, given in (("dq_weight", dq_weight, q_weight), ("dk_weight", dk_weight, k_weight)):
         if w is not None:
             if given is None:
                 raise ValueError(f"{name} is wanted of a weight that is None")
             _check(w, name, (d,), dev, given.dtype)
-            need = qkv_norm_rope_grad_workspace(n, heads[0], max(heads[1:]), d)
-    ws = _workspace(workspace, need, dev)
-    L = _lib
-    _call_on(dev, "eg2_launch_qkv_norm_rope_grad", L.EgQkvNormRopeGrad(
-        L.P3(*[a[0] for a in dx]), L.P2(_p(dq_weight), _p(dk_weight)), L.P3(*[a[0] for a in g]),
-        L.P3(*[a[0] for a in x]), L.P2(_p(q_weight), _p(k_weight)), _p(rope_cos), _p(rope_sin), _p(pos), _p(ws),
-        ws.numel() * ws.element_size(), L.Strides3(*[a[1] for a in dx]), L.Strides3(*[a[1] for a in g]),
-        L.Strides3(*[a[1] for a in x]), n, *heads, d, positions, code, wtype, eps, int(accumulate)))
-
-
-_ACTS = {"gelu_tanh": 0, "silu": 1}
+            need = qkv_norm_rope_grad_workspace(n, hq, max(hk, hv), d)
+    ws = _workspace(workspace, need, dev) if need else (0, 0, None)
+    _qkv_norm_rope_grad(dev, *dx, _ptr(dq_weight), _ptr(dk_weight), *g, *x, _ptr(q_weight), _ptr(k_weight),
+                        rope_cos.data_ptr(), rope_sin.data_ptr(), pos.data_ptr(), ws[0], ws[1], *dxs, *gs, *xs,
+                        *sizes, eps, bool(accumulate))
 
 
 def _glu_args(x, w_gate, w_up, act):
     if act not in _ACTS:
         raise ValueError(f"act {act!r}: expected one of {sorted(_ACTS)}")
-    dev = x.device
-    _check(x, "x", (None, None))
-    n, k = x.shape
+    (n, k), dev, xs = _lead(x, "x", 2)
+    dtype = x.dtype
     code = _type(x, "x")
     if code == 0:
         raise ValueError("x is torch.float32: expected float16 or bfloat16")
-    _check(w_gate, "w_gate", (None, k), dev, x.dtype)
     m = w_gate.shape[0]
-    _check(w_up, "w_up", (m, k), dev, x.dtype)
+    gs = _check(w_gate, "w_gate", (m, k), dev, dtype)
+    us = _check(w_up, "w_up", (m, k), dev, dtype)
     if k % 8 or m % 8 or not k or not m:
         raise ValueError(f"k = {k}, m = {m}: expected multiples of 8")
-    return n, k, m, dev, code
+    return n, k, m, dev, dtype, code, (xs[0], gs[0], us[0])
 
 
 def glu(out, x, w_gate, w_up, act="gelu_tanh"):
     """out = act(x w_gate^T) * (x w_up^T): x [n][k], weights [m][k], out [n][m], float16 or bfloat16.
 
     act is "gelu_tanh" or "silu"; k and m are multiples of 8, rows 16-byte aligned."""
-    n, k, m, dev, code = _glu_args(x, w_gate, w_up, act)
-    _check(out, "out", (n, m), dev, x.dtype)
-    _call_on(dev, "eg2_launch_glu", _lib.EgGlu(
-        _p(out), _p(x), _p(w_gate), _p(w_up), out.stride(0), x.stride(0), w_gate.stride(0), w_up.stride(0), n, k, m,
-        code, _ACTS[act]))
+    n, k, m, dev, dtype, code, strides = _glu_args(x, w_gate, w_up, act)
+    out_stride = _check(out, "out", (n, m), dev, dtype)[0]
+    _glu(dev, out.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), out_stride, *strides, n, k, m, code,
+         _ACTS[act])
 
 
 def glu_grad_workspace(n, k, m) -> int:
@@ -348,25 +389,18 @@ def glu_grad(dx, dw_gate, dw_up, dout, x, w_gate, w_up, act="gelu_tanh", accumul
     The weights' gradients are of x's type or float32; with accumulate they are
     float32 and added to.  Nothing is kept from the forward pass: the
     projections are computed again."""
-    n, k, m, dev, code = _glu_args(x, w_gate, w_up, act)
-    _check(dout, "dout", (n, m), dev, x.dtype)
-    if dx is not None:
-        _check(dx, "dx", (n, k), dev, x.dtype)
-    dw_code = code
-    for name, w in (("dw_gate", dw_gate), ("dw_up", dw_up)):
-        if w is not None:
-            _check(w, name, (m, k), dev)
-            dw_code = _type(w, name)
-    if dw_gate is not None and dw_up is not None and dw_gate.dtype != dw_up.dtype:
-        raise ValueError(f"dw_gate is {dw_gate.dtype}, dw_up {dw_up.dtype}: expected one type")
-    if dw_code not in (0, code) or (accumulate and dw_code != 0 and not (dw_gate is None and dw_up is None)):
-        raise ValueError("weight gradients are float32 or x's type, float32 with accumulate")
+    n, k, m, dev, dtype, code, strides = _glu_args(x, w_gate, w_up, act)
+    dout_stride = _check(dout, "dout", (n, m), dev, dtype)[0]
+    dw_type = dw_gate.dtype if dw_gate is not None else dw_up.dtype if dw_up is not None else dtype
+    if dw_type not in (torch.float32, dtype) or (accumulate and dw_type != torch.float32):
+        raise ValueError(f"weight gradients are {dw_type}: expected float32" + ("" if accumulate else f" or {dtype}"))
+    dx_stride = 0 if dx is None else _check(dx, "dx", (n, k), dev, dtype)[0]
+    dg_stride = 0 if dw_gate is None else _check(dw_gate, "dw_gate", (m, k), dev, dw_type)[0]
+    du_stride = 0 if dw_up is None else _check(dw_up, "dw_up", (m, k), dev, dw_type)[0]
     ws = _workspace(workspace, glu_grad_workspace(n, k, m), dev)
-    st = lambda t: 0 if t is None else t.stride(0)
-    _call_on(dev, "eg2_launch_glu_grad", _lib.EgGluGrad(
-        _p(dx), _p(dw_gate), _p(dw_up), _p(dout), _p(x), _p(w_gate), _p(w_up), _p(ws), ws.numel() * ws.element_size(),
-        st(dx), st(dw_gate), st(dw_up), dout.stride(0), x.stride(0), w_gate.stride(0), w_up.stride(0), n, k, m, code,
-        _ACTS[act], dw_code, int(accumulate and dw_code == 0)))
+    _glu_grad(dev, _ptr(dx), _ptr(dw_gate), _ptr(dw_up), dout.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
+              w_up.data_ptr(), ws[0], ws[1], dx_stride, dg_stride, du_stride, dout_stride, *strides, n, k, m, code,
+              _ACTS[act], _TYPES[dw_type], bool(accumulate))
 
 
 def repack_q8(blocks, rows, k, codes, scales):

@@ -107,6 +107,27 @@ def test_qkv_norm_rope_refuses_pointers_and_strides(L):
         assert qkv_grad(L, **kw) == INVALID
 
 
+def test_packed_parameters_have_the_struct_layout(eg2, L):
+    """The Python entry points pack parameters as the C structs lay them out."""
+    ops = importlib.import_module("embeddinggemma2-amdkfd_b200.ops")
+    for op, cls in ((ops._embed_rows, L.EgEmbedRows), (ops._embed_rows_grad, L.EgEmbedRowsGrad),
+                    (ops._qkv_norm_rope, L.EgQkvNormRope), (ops._qkv_norm_rope_grad, L.EgQkvNormRopeGrad),
+                    (ops._glu, L.EgGlu), (ops._glu_grad, L.EgGluGrad)):
+        flat, rows, i = [], {}, 1
+        for name, t in cls._fields_:
+            count = C.sizeof(t) // (4 if t in (C.c_uint, C.c_float) else 8)
+            rows[name] = list(range(i, i + count))
+            flat += rows[name]
+            i += count
+        params = op.pack(*flat)
+        assert len(params) == C.sizeof(cls), op.name
+        got = cls.from_buffer_copy(params)
+        for name, t in cls._fields_:
+            v = getattr(got, name)
+            v = [x for y in v for x in (y if hasattr(y, "__len__") else [y])] if hasattr(v, "__len__") else [v]
+            assert v == rows[name], (op.name, name)
+
+
 def test_workspace_sizes(L):
     lib = L.load()
     for n in (1, 7, 2048, 32767, 32768, 262144, 262145, 1_000_000):
@@ -114,8 +135,8 @@ def test_workspace_sizes(L):
             size = lib.eg2_embed_rows_grad_workspace(n, d)
             chunks = -(-n // (32 if n >= 32768 else 8))
             assert size >= 16 * n + 8 * chunks * d and size % 256 == 0
-    assert lib.eg2_qkv_norm_rope_grad_workspace(1, 4, 2, 256) == 8 * 2 * 256 * 4
-    assert lib.eg2_qkv_norm_rope_grad_workspace(100000, 4, 2, 256) == 1024 * 2 * 256 * 4
+    assert lib.eg2_qkv_norm_rope_grad_workspace(1, 4, 2, 256) == 8 * 256 * 4
+    assert lib.eg2_qkv_norm_rope_grad_workspace(100000, 4, 2, 256) == 1024 * 256 * 4
 
 
 def test_python_entry_points_refuse_cpu_tensors(eg2):
