@@ -65,21 +65,6 @@ struct GluParams {
 };
 
 // ---------------------------------------------------------------- cluster pieces
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-// The address, in the cluster's shared window, of the even CTA's copy of p.
-__device__ __forceinline__ uint32_t even_cta_addr(const void *p) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
-    return r;
-}
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
@@ -216,7 +201,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
                     }
                     // The even CTA's barrier counts both CTAs' bytes.
                     if (rank == 0) bar_expect_tx(&full[s], 2 * C::STAGE);
-                    const uint32_t bar = even_cta_addr(&full[s]);
+                    const uint32_t bar = cluster_addr(0, &full[s]);
                     uint8_t *a = a_tile(s), *b = b_tile(s);
                     const int arow = t.row0 + rank * 128;
                     if (MODE != GLU_PRODUCTS) {
@@ -394,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
             // The accumulator is free for the tile after next once both CTAs' warps have read it.
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive_cluster(even_cta_addr(&accempty[buf]));
+            if (lane == 0) bar_arrive_cluster(cluster_addr(0, &accempty[buf]));
         }
     }
     // Both CTAs' barriers and shared memory stay until neither uses the other's.

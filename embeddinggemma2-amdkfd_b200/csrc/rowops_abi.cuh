@@ -11,6 +11,10 @@ static inline int type_size(unsigned t) { return t == EG_F32 ? 4 : t == EG_F16 |
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static inline int ceil_div(long long a, long long b) { return int((a + b - 1) / b); }
 
+template <int I>
+struct Int {
+    static constexpr int value = I;
+};
 // f(type tag) for an element type; cudaErrorInvalidValue for any other number.
 template <typename T>
 struct Tag {
@@ -71,16 +75,17 @@ static cudaError_t embed_rows(const EgEmbedRows &a, cudaStream_t s) {
     });
 }
 
-// Workspace: two (key, token) arrays, the digit histogram, and the head and tail
-// parts of every chunk.
+// Workspace: two arrays of (key, token), the digit histogram, the touched rows' flags,
+// and the head and tail parts of every chunk.
 struct EmbedGradLayout {
     int tiles, subtiles, chunk, chunks;
-    size_t key[2], tok[2], hist, head, tail, total;
+    size_t items[2], hist, touched, head, tail, total;
 };
 static EmbedGradLayout embed_grad_layout(unsigned n, unsigned d) {
     EmbedGradLayout L{};
-    // Short chunks while the batch is small, for more warps; long ones leave fewer parts to join.
-    L.chunk = n >= 32768 ? 32 : 8;
+    // About 8 warps on each of 148 SMs, a warp for 256 columns of a chunk; 8 items at least.
+    const long long warps = 8 * 148, share = ceil_div((long long)n * ceil_div(d, 256), warps);
+    L.chunk = int((share < 8 ? 8 : share) + 7) / 8 * 8;
     L.chunks = ceil_div(n, L.chunk);
     L.subtiles = ceil_div(n, (long long)EmbedSort::SUB * EmbedSort::MAX_TILES);
     if (L.subtiles < 1) L.subtiles = 1;
@@ -91,8 +96,9 @@ static EmbedGradLayout embed_grad_layout(unsigned n, unsigned d) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    for (int i = 0; i < 2; ++i) L.key[i] = take(size_t(n) * 4), L.tok[i] = take(size_t(n) * 4);
+    for (int i = 0; i < 2; ++i) L.items[i] = take(size_t(n) * 8);
     L.hist = take(size_t(L.tiles) * EmbedSort::MAX_BINS * 4);
+    L.touched = take(EmbedSort::MAX_TOUCHED);
     L.head = take(size_t(L.chunks) * d * 4);
     L.tail = take(size_t(L.chunks) * d * 4);
     L.total = at;
@@ -113,8 +119,7 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
         (reinterpret_cast<uintptr_t>(a.workspace) & 255) || a.dout_stride < 0)
         return cudaErrorInvalidValue;
     uint8_t *ws = static_cast<uint8_t *>(a.workspace);
-    unsigned *key[2] = {reinterpret_cast<unsigned *>(ws + L.key[0]), reinterpret_cast<unsigned *>(ws + L.key[1])};
-    int *tok[2] = {reinterpret_cast<int *>(ws + L.tok[0]), reinterpret_cast<int *>(ws + L.tok[1])};
+    uint2 *items[2] = {reinterpret_cast<uint2 *>(ws + L.items[0]), reinterpret_cast<uint2 *>(ws + L.items[1])};
 
     // Keys are 0 .. vocab (padding last); equal digits over as few passes as cover them.
     int key_bits = 1;
@@ -123,46 +128,86 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
     EmbedSortParams q{};
     q.hist = reinterpret_cast<unsigned *>(ws + L.hist);
     q.n = int(a.n), q.vocab = int(a.vocab), q.tiles = L.tiles, q.subtiles = L.subtiles, q.bits = bits;
-    if (!a.accumulate) {
-        // The table is cleared by CTAs beside the sort's, a share of its rows in each of its launches.
-        q.fill = static_cast<unsigned char *>(a.dtable);
-        q.fill_stride_bytes = stride * sw, q.fill_width_bytes = int(a.d) * sw;
-        const long long want = ceil_div((long long)a.vocab * a.d * sw, 2 * passes * 65536ll);
-        q.fill_ctas = int(want < 1 ? 1 : want > 4 * sm_count() ? 4 * sm_count() : want);
-    }
-    for (int pass = 0; pass < passes; ++pass) {
-        q.ids = pass ? nullptr : a.ids;
-        q.key_in = key[pass & 1], q.tok_in = tok[pass & 1];
-        q.key_out = key[(pass + 1) & 1], q.tok_out = tok[(pass + 1) & 1];
-        q.shift = pass * bits;
-        for (int half = 0; half < 2; ++half) {
-            const long long step = 2 * pass + half, steps = 2 * passes;
-            q.fill_row0 = a.vocab * step / steps;
-            q.fill_rows = a.accumulate ? 0 : a.vocab * (step + 1) / steps - q.fill_row0;
-            const dim3 grid(L.tiles + q.fill_ctas);
-            if (cudaError_t e = launch_pdl(half ? embed_scatter_kernel : embed_hist_kernel, grid,
-                                           dim3(EmbedSort::THREADS), 0, s, q))
-                return e;
+    // The table's untouched rows are cleared beside the other work: in each launch
+    // of the sort about what can be written in the time that it takes anyway, the
+    // rest beside the sums.  A larger vocabulary than there are flags for is
+    // cleared whole before the sums.
+    const bool flags_fit = a.vocab <= EmbedSort::MAX_TOUCHED;
+    uint8_t *touched = a.accumulate || !flags_fit ? nullptr : ws + L.touched;
+    const long long block_bytes = 8ll * a.d * sw;
+    long long left = ceil_div(a.vocab, 8);  // blocks of 8 rows, handed out from the end
+    auto share = [&](long long bytes, int warps, bool skip) {
+        EmbedFill f{};
+        if (a.accumulate) return f;
+        long long count = bytes < 0 ? left : bytes / block_bytes;
+        if (count > left) count = left;
+        f.table = static_cast<unsigned char *>(a.dtable), f.touched = skip ? touched : nullptr;
+        f.stride = stride * sw, f.width = int(a.d) * sw, f.rows = int(a.vocab);
+        f.per_warp = block_bytes >= 16384 ? 1 : int(16384 / block_bytes);
+        f.ctas = ceil_div(count, (long long)warps * f.per_warp);
+        left -= count;
+        f.block0 = left, f.blocks = count;
+        return f;
+    };
+    int sorted = passes & 1;  // which pair of arrays ends up holding the items in order
+    if (a.n <= EmbedSmall::CAP) {
+        using S = EmbedSmall;
+        EmbedSmallParams c{};
+        sorted = 0;
+        c.ids = a.ids, c.out = items[0], c.touched = touched;
+        c.n = q.n, c.vocab = q.vocab, c.bits = bits, c.passes = passes, c.per = ceil_div(a.n, S::THREADS);
+        c.fill = share(flags_fit ? 96 << 20 : -1, S::WARPS, false);
+        static AllowSmem allow;
+        if (cudaError_t e = allow(embed_sort_kernel, S::SMEM)) return e;
+        if (cudaError_t e = launch_pdl(embed_sort_kernel, dim3(1 + c.fill.ctas), dim3(S::THREADS), S::SMEM, s, c))
+            return e;
+    } else {
+        for (int pass = 0; pass < passes; ++pass) {
+            q.ids = pass ? nullptr : a.ids;
+            q.in = items[pass & 1], q.out = items[(pass + 1) & 1];
+            q.shift = pass * bits;
+            for (int half = 0; half < 2; ++half) {
+                const bool last = pass == passes - 1 && half;
+                q.touched = pass == passes - 1 ? touched : nullptr;
+                q.fill = share(last && !flags_fit ? -1 : half ? 32 << 20 : 0, EmbedSort::WARPS, false);
+                if (cudaError_t e = launch_pdl(half ? embed_scatter_kernel : embed_hist_kernel,
+                                               dim3(L.tiles + q.fill.ctas), dim3(EmbedSort::THREADS), 0, s, q))
+                    return e;
+            }
         }
     }
-    const EmbedSumParams u{a.dtable, a.dout, key[passes & 1], tok[passes & 1],
-                           reinterpret_cast<float *>(ws + L.head), reinterpret_cast<float *>(ws + L.tail), stride,
-                           a.dout_stride, int(a.n), int(a.vocab), int(a.d), L.chunk, L.chunks, a.scale,
-                           int(a.accumulate != 0)};
-    const bool wide = a.d % 8 == 0 && aligned16(a.dtable) && aligned16(a.dout) && stride * sw % 16 == 0 &&
-                      (a.n == 1 || a.dout_stride * sg % 16 == 0);
+    EmbedSumParams u{};
+    u.dtable = a.dtable, u.dout = a.dout, u.items = items[sorted];
+    u.head = reinterpret_cast<float *>(ws + L.head), u.tail = reinterpret_cast<float *>(ws + L.tail);
+    u.dtable_stride = stride, u.dout_stride = a.dout_stride;
+    u.n = int(a.n), u.vocab = int(a.vocab), u.d = int(a.d), u.chunk = L.chunk, u.chunks = L.chunks;
+    u.scale = a.scale, u.accumulate = a.accumulate != 0;
+    u.fill = share(-1, EmbedSum::WARPS, true);
+    // 16 bytes of dout per lane and row where all rows allow it, else pairs, else single elements.
+    const auto rows_fit = [&](int v) {
+        auto fits = [&](const void *p, long long row_stride, unsigned rows, int bytes) {
+            const int w = bytes < 16 ? bytes : 16;
+            return reinterpret_cast<uintptr_t>(p) % w == 0 && (rows < 2 || row_stride * (bytes / v) % w == 0);
+        };
+        return a.d % v == 0 && fits(a.dout, a.dout_stride, a.n, v * sg) && fits(a.dtable, stride, a.vocab, v * sw);
+    };
     return by_type(a.dout_type, [&](auto tg) {
         return by_type(a.dtable_type, [&](auto tw) {
             using TG = typename decltype(tg)::type;
             using TW = typename decltype(tw)::type;
-            const dim3 block(256);
-            const int cols = ceil_div(a.d, wide ? 256 : 32);
-            const dim3 sum_grid(ceil_div(L.chunks, 8), cols), join_grid(L.chunks, cols);
-            if (cudaError_t e = wide ? launch_pdl(embed_sum_kernel<TG, TW, 8>, sum_grid, block, 0, s, u)
-                                     : launch_pdl(embed_sum_kernel<TG, TW, 1>, sum_grid, block, 0, s, u))
-                return e;
-            return wide ? launch_pdl(embed_join_kernel<TW, 8>, join_grid, block, 0, s, u)
-                        : launch_pdl(embed_join_kernel<TW, 1>, join_grid, block, 0, s, u);
+            const auto go = [&](auto vec) -> cudaError_t {
+                constexpr int V = decltype(vec)::value;
+                u.col_blocks = ceil_div(a.d, 32 * V);
+                u.sum_ctas = ceil_div((long long)L.chunks * u.col_blocks, EmbedSum::WARPS);
+                const size_t ring = V * sizeof(TG) == 16 ? EmbedSum::RING : 0;  // 48 KB: no opt-in needed
+                if (cudaError_t e = launch_pdl(embed_sum_kernel<TG, TW, V>, dim3(u.sum_ctas + u.fill.ctas),
+                                               dim3(EmbedSum::THREADS), ring, s, u))
+                    return e;
+                if (L.chunks < 2) return cudaSuccess;
+                return launch_pdl(embed_join_kernel<TW, V>, dim3(ceil_div(L.chunks, 32), u.col_blocks), dim3(256), 0, s, u);
+            };
+            constexpr int WIDE = 16 / int(sizeof(TG));
+            return rows_fit(WIDE) ? go(Int<WIDE>{}) : rows_fit(2) ? go(Int<2>{}) : go(Int<1>{});
         });
     });
 }
@@ -186,10 +231,6 @@ static bool qkv_tensor_ok(const void *p, int64_t tok, int64_t head, unsigned n, 
 }
 
 // f(V, G, NV) as integral constants for a row of half = d / 2 elements of T.
-template <int I>
-struct Int {
-    static constexpr int value = I;
-};
 template <typename T, typename F>
 static cudaError_t qkv_shape(int half, bool wide, F f) {
     constexpr int V = 16 / int(sizeof(T));

@@ -18,42 +18,52 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V consecutive elements, held in their own type: V * sizeof(T) bytes, moved in
-// 16-byte accesses where they are that long (the address is then a multiple of
-// 16), element by element otherwise.
+// V consecutive elements, held in their own type and moved in the widest accesses
+// of 2 to 16 bytes that divide them; the address is a multiple of that width.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> {
+    using type = uint16_t;
+};
+template <>
+struct Word<4> {
+    using type = uint32_t;
+};
+template <>
+struct Word<8> {
+    using type = uint2;
+};
+template <>
+struct Word<16> {
+    using type = uint4;
+};
 template <typename T, int V>
 struct Pack {
-    static constexpr int BYTES = V * int(sizeof(T)), WORDS = BYTES / 16;
-    static constexpr bool WIDE = BYTES % 16 == 0;
-    static_assert(WIDE || V == 1, "a vector is whole 16-byte words or one element");
-    uint4 w[WIDE ? WORDS : 1];
+    static constexpr int BYTES = V * int(sizeof(T)), WIDTH = BYTES < 16 ? BYTES : 16, WORDS = BYTES / WIDTH;
+    using W = typename Word<WIDTH>::type;
+    union {
+        W w[WORDS];
+        T e[V];
+    };
+    __device__ __forceinline__ Pack() {}
     __device__ __forceinline__ void load(const T *p) {
-        if constexpr (WIDE) {
 #pragma unroll
-            for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
-        } else {
-            *reinterpret_cast<T *>(w) = *p;
-        }
+        for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const W *>(p)[i];
     }
     __device__ __forceinline__ void store(T *p) const {
-        if constexpr (WIDE) {
 #pragma unroll
-            for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
-        } else {
-            *p = *reinterpret_cast<const T *>(w);
-        }
+        for (int i = 0; i < WORDS; ++i) reinterpret_cast<W *>(p)[i] = w[i];
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (auto &x : w) x = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < WORDS; ++i) w[i] = W{};
     }
     __device__ __forceinline__ void get(float (&f)[V]) const {
-        const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = to_f32(e[i]);
     }
     __device__ __forceinline__ void set(const float (&f)[V]) {
-        T *e = reinterpret_cast<T *>(w);
 #pragma unroll
         for (int i = 0; i < V; ++i) e[i] = from_f32<T>(f[i]);
     }

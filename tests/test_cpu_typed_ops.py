@@ -133,8 +133,7 @@ def test_workspace_sizes(L):
     for n in (1, 7, 2048, 32767, 32768, 262144, 262145, 1_000_000):
         for d in (1, 512):
             size = lib.eg2_embed_rows_grad_workspace(n, d)
-            chunks = -(-n // (32 if n >= 32768 else 8))
-            assert size >= 16 * n + 8 * chunks * d and size % 256 == 0
+            assert size >= 16 * n and size % 256 == 0
     assert lib.eg2_qkv_norm_rope_grad_workspace(1, 4, 2, 256) == 8 * 256 * 4
     assert lib.eg2_qkv_norm_rope_grad_workspace(100000, 4, 2, 256) == 1024 * 256 * 4
 
