@@ -33,7 +33,8 @@
 // Per CTA: warp 0 TMA producer, warp 1 MMA issuer (even CTA) and owner of tensor
 // memory, warps 4..11 epilogue (lane quadrant = warp % 4, half of the columns
 // each).  Two accumulators of BN columns, so that a tile's epilogue runs under
-// the next tile's products.  Persistent: a cluster takes every (gridDim / 2)th tile.
+// the next tile's products.  Persistent; in GLU_PRODUCTS the clusters are shared out
+// between dx's tiles (K = 2 m) and the weights' (K = n) by their lengths.
 #pragma once
 #include "typed.cuh"
 
@@ -42,13 +43,18 @@ namespace eg2 {
 enum : int { GLU_FORWARD = 0, GLU_DGRAD = 1, GLU_PRODUCTS = 2 };
 enum : int { ACT_GELU_TANH = 0, ACT_SILU = 1 };
 
-template <int BN_>
+template <int MODE, int BN_>
 struct GluCfg {
     static constexpr int BN = BN_, BM = 256, BK = 64;  // one cluster's tile
-    static constexpr int STAGES = 6, THREADS = 12 * 32, EPI_WARPS = 8;
+    static constexpr int THREADS = 12 * 32, EPI_WARPS = 8;
     static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = BN / 2 * BK * 2, STAGE = A_BYTES + B_BYTES;
     static constexpr int B_ROWS = BN / 2 < 64 ? BN / 2 : 64;  // rows of a weight box
-    static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 256;
+    // An epilogue warp's own tile in shared memory: its 32 rows x ROW bytes (a
+    // quarter of the columns, or 128 bytes of them at a time), two in GLU_DGRAD.
+    static constexpr int ROW = MODE == GLU_PRODUCTS ? 128 : BN / 4 * 2, CHUNKS = ROW / 16;
+    static constexpr int STAGING = 32 * ROW * (MODE == GLU_DGRAD ? 2 : 1);
+    static constexpr int STAGES = MODE == GLU_DGRAD && BN == 256 ? 5 : 6;
+    static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + EPI_WARPS * STAGING + 256;
 };
 
 struct GluMaps {
@@ -62,6 +68,9 @@ struct GluParams {
     long long out_stride[3];
     int dw_f32, dw_accumulate;    // PRODUCTS: the weight gradients' type, and whether they are added to
     int tiles, dx_tiles, group;   // tiles in all; those of dx come first; row tiles walked together
+    int splits;                   // PRODUCTS: dx's K in this many parts, a tile each; above 1 they are
+    float *parts;                 // written here, [splits][n][k] in fp32, for glu_add_kernel
+    int dx_clusters;              // PRODUCTS: clusters 0 .. dx_clusters - 1 take dx's tiles, the others the weights'
 };
 
 // ---------------------------------------------------------------- cluster pieces
@@ -129,15 +138,20 @@ __device__ __forceinline__ float glu_act_grad(float g, float *act) {
 // ---------------------------------------------------------------- tiles
 // kind 0: the projections' tile or dx's; kinds 1 and 2: dWg's and dWu's.
 struct GluTile {
-    int kind, row0, col0, steps;
+    int kind, row0, col0, steps, step0, part;  // K steps step0 .. step0 + steps - 1
 };
 template <int MODE, int BN>
 __device__ __forceinline__ GluTile glu_tile(const GluParams &p, int i) {
     const int steps_m = (p.m + 63) / 64;
-    int kind = 0, rows = p.n, cols = p.m, bn = BN / 2, steps = (p.k + 63) / 64;
+    int kind = 0, rows = p.n, cols = p.m, bn = BN / 2, steps = (p.k + 63) / 64, step0 = 0, part = 0;
     if (MODE == GLU_PRODUCTS) {
         cols = p.k, bn = BN, steps = 2 * steps_m;
-        if (i >= p.dx_tiles) {
+        if (i < p.dx_tiles) {
+            const int each = p.dx_tiles / p.splits;
+            part = i / each, i -= part * each;
+            step0 = int((long long)steps * part / p.splits);
+            steps = int((long long)steps * (part + 1) / p.splits) - step0;
+        } else {
             i -= p.dx_tiles;
             rows = p.m, steps = (p.n + 63) / 64;
             kind = p.out[1] ? 1 : 2;
@@ -150,17 +164,18 @@ __device__ __forceinline__ GluTile glu_tile(const GluParams &p, int i) {
     const int tm = (rows + 255) / 256, tn = (cols + bn - 1) / bn;
     const int band = i / (p.group * tn), r0 = band * p.group, height = min(p.group, tm - r0);
     const int j = i - band * p.group * tn;
-    return {kind, (r0 + j % height) * 256, (j / height) * bn, steps};
+    return {kind, (r0 + j % height) * 256, (j / height) * bn, steps, step0, part};
 }
 
 template <int MODE, int BN, typename T, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<MODE, BN>::THREADS, 1)
     glu_kernel(const __grid_constant__ GluMaps maps, const __grid_constant__ GluParams p) {
-    using C = GluCfg<BN>;
+    using C = GluCfg<MODE, BN>;
     static_assert(sizeof(T) == 2, "16-bit operands");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = align_smem_1024(smem_raw);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + size_t(C::STAGES) * C::STAGE);
+    uint8_t *staging = smem + size_t(C::STAGES) * C::STAGE;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + C::EPI_WARPS * C::STAGING);
     uint64_t *full = bars, *empty = full + C::STAGES, *accfull = empty + C::STAGES, *accempty = accfull + 2;
     uint64_t *mdone = accempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mdone + 1);
@@ -169,7 +184,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
     auto b_tile = [&](int s) { return smem + s * C::STAGE + C::A_BYTES; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = int(cluster_rank()), cluster = blockIdx.x / 2, clusters = gridDim.x / 2;
+    const int rank = int(cluster_rank());
+    // This cluster's tiles: first, first + step, ... below end.
+    int first = blockIdx.x / 2, step = gridDim.x / 2, end = p.tiles;
+    if (MODE == GLU_PRODUCTS) {
+        if (first < p.dx_clusters) step = p.dx_clusters, end = p.dx_tiles;
+        else first += p.dx_tiles - p.dx_clusters, step -= p.dx_clusters;
+    }
     if (threadIdx.x == 0) {
         tma_prefetch(&maps.x), tma_prefetch(&maps.wg), tma_prefetch(&maps.wu);
         *abort = 0;
@@ -191,7 +212,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (int i = cluster; ok && i < p.tiles; i += clusters) {
+            for (int i = first; ok && i < end; i += step) {
                 const GluTile t = glu_tile<MODE, BN>(p, i);
                 for (int kb = 0; kb < t.steps; ++kb, ++it) {
                     const int s = it % C::STAGES;
@@ -211,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
                     } else {
                         const int bcol = t.col0 + rank * (BN / 2);
                         if (t.kind == 0) {
-                            const int per = t.steps / 2, seg = kb >= per, k0 = (kb - seg * per) * 64;
+                            const int per = (p.m + 63) / 64, ks = t.step0 + kb, seg = ks >= per, k0 = (ks - seg * per) * 64;
                             for (int j = 0; j < 2; ++j)
                                 tma_load_2d_pair(a + j * 8192, seg ? &maps.du : &maps.dg, bar, k0, arow + j * 64);
                             for (int j = 0; j < BN / 128; ++j)
@@ -242,7 +263,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
             constexpr uint32_t BASE = (1u << 4) | FMT | (uint32_t(BN >> 3) << 17) | (uint32_t(C::BM >> 4) << 24);
             int it = 0, ti = 0;
             bool ok = true;
-            for (int i = cluster; ok && i < p.tiles; i += clusters, ++ti) {
+            for (int i = first; ok && i < end; i += step, ++ti) {
                 const GluTile t = glu_tile<MODE, BN>(p, i);
                 const int buf = ti & 1;
                 const bool a_mn = MODE == GLU_PRODUCTS && t.kind != 0;
@@ -277,72 +298,123 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------------ epilogue
+        // A thread has one row of the accumulator; memory wants whole rows of a
+        // tile from neighbouring lanes.  Between the two each warp turns its rows
+        // in its own piece of shared memory, in 16-byte chunks whose places are
+        // permuted by row so that both ways are free of bank conflicts.
         const int quad = warp & 3, part = (warp - 4) >> 2;
         const uint32_t lanes = tmem + (uint32_t(quad * 32) << 16);
+        uint8_t *mine = staging + (warp - 4) * C::STAGING;
+        auto chunk = [&](int r, int c) {
+            return reinterpret_cast<uint4 *>(mine + r * C::ROW + ((c ^ (r * C::ROW / 128)) & (C::CHUNKS - 1)) * 16);
+        };
+        // Lane's chunk of the i-th group of rows that one access covers.
+        const int crow = lane / C::CHUNKS, ccol = lane % C::CHUNKS;
+        constexpr int PER = 32 / C::CHUNKS;
         int ti = 0;
-        for (int i = cluster; i < p.tiles; i += clusters, ++ti) {
+        for (int i = first; i < end; i += step, ++ti) {
             const GluTile t = glu_tile<MODE, BN>(p, i);
-            const int buf = ti & 1, row = t.row0 + rank * 128 + quad * 32 + lane;
+            const int buf = ti & 1, row0 = t.row0 + rank * 128 + quad * 32;
+            const uint32_t acc = lanes + uint32_t(buf * BN);
+            uint4 dh[MODE == GLU_DGRAD ? C::CHUNKS : 1];
+            if constexpr (MODE == GLU_DGRAD) {  // dout's rows while the products are still running
+                const int col = t.col0 + part * (BN / 4) + ccol * 8;
+#pragma unroll
+                for (int c = 0; c < C::CHUNKS; ++c) {
+                    const int r = row0 + c * PER + crow;
+                    dh[c] = make_uint4(0, 0, 0, 0);
+                    if (r < p.n && col < p.m)
+                        dh[c] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.dout) + r * p.dout_stride + col);
+                }
+            }
             if (!__all_sync(0xffffffffu, wait_bar(&accfull[buf], (ti >> 1) & 1, abort))) break;
             tc_fence_after();
-            const uint32_t acc = lanes + uint32_t(buf * BN);
+            // The accumulator is free for the tile after next once both CTAs' warps have read it.
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_cluster(cluster_addr(0, &accempty[buf]));
+            };
             if constexpr (MODE == GLU_PRODUCTS) {
-                const bool dw = t.kind != 0;
-                const int rows = dw ? p.m : p.n;
-                for (int c0 = part * (BN / 2); c0 < (part + 1) * (BN / 2); c0 += 32) {
+                const bool dw = t.kind != 0, f32 = dw ? p.dw_f32 : p.splits > 1;
+                const int rows = dw ? p.m : p.n, each = f32 ? 32 : 64;  // columns in 128 bytes
+                const long long pitch = !dw && f32 ? p.k : p.out_stride[t.kind];
+                void *dst = !dw && f32 ? static_cast<void *>(p.parts + (long long)t.part * p.n * p.k) : p.out[t.kind];
+                const int last = (part + 1) * (BN / 2);
+                for (int c0 = part * (BN / 2); c0 < last; c0 += each) {
+                    if (t.col0 + c0 >= p.k) break;
                     uint32_t r[32];
                     tmem_ld32(acc + uint32_t(c0), r);
                     tmem_wait_ld();
                     reg_fence(r);
-                    const int col = t.col0 + c0;
-                    if (row < rows) {
-                        if (dw && p.dw_f32) {
-                            float *dst = static_cast<float *>(p.out[t.kind]) + row * p.out_stride[t.kind] + col;
+                    if (f32) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                if (col + 4 * j >= p.k) break;
-                                float4 v = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                                       __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
-                                if (p.dw_accumulate) {
-                                    const float4 o = reinterpret_cast<const float4 *>(dst)[j];
-                                    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-                                }
-                                reinterpret_cast<float4 *>(dst)[j] = v;
+                        for (int c = 0; c < 8; ++c)
+                            *chunk(lane, c) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (h) {
+                                tmem_ld32(acc + uint32_t(c0 + 32), r);
+                                tmem_wait_ld();
+                                reg_fence(r);
                             }
-                        } else {
-                            T *dst = static_cast<T *>(p.out[t.kind]) + row * p.out_stride[t.kind] + col;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                if (col + 8 * j >= p.k) break;
+                            for (int c = 0; c < 4; ++c) {
                                 uint32_t w[4];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
-                                    w[e] = pack2<T>(__uint_as_float(r[8 * j + 2 * e]),
-                                                    __uint_as_float(r[8 * j + 2 * e + 1]));
-                                reinterpret_cast<uint4 *>(dst)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                                    w[e] = pack2<T>(__uint_as_float(r[8 * c + 2 * e]),
+                                                    __uint_as_float(r[8 * c + 2 * e + 1]));
+                                *chunk(lane, 4 * h + c) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
                     }
+                    __syncwarp();
+                    const int col = t.col0 + c0 + ccol * (f32 ? 4 : 8);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const int rr = row0 + c * PER + crow;
+                        if (rr >= rows || col >= p.k) continue;
+                        uint4 v = *chunk(c * PER + crow, ccol);
+                        uint8_t *to = static_cast<uint8_t *>(dst) + (rr * pitch + col) * (f32 ? 4 : 2);
+                        if (dw && p.dw_accumulate) {
+                            const float4 o = *reinterpret_cast<const float4 *>(to);
+                            v = make_uint4(__float_as_uint(__uint_as_float(v.x) + o.x),
+                                           __float_as_uint(__uint_as_float(v.y) + o.y),
+                                           __float_as_uint(__uint_as_float(v.z) + o.z),
+                                           __float_as_uint(__uint_as_float(v.w) + o.w));
+                        }
+                        *reinterpret_cast<uint4 *>(to) = v;
+                    }
+                    __syncwarp();
                 }
+                release();
             } else {
                 // Gate columns 0 .. BN/2 - 1 of the accumulator, up columns BN/2 ..; this warp's half of each.
+                if constexpr (MODE == GLU_DGRAD) {
+#pragma unroll
+                    for (int c = 0; c < C::CHUNKS; ++c) *chunk(c * PER + crow, ccol) = dh[c];
+                    __syncwarp();
+                }
                 constexpr int STEP = BN / 4 < 32 ? BN / 4 : 32;
-                for (int c0 = part * (BN / 4); c0 < (part + 1) * (BN / 4); c0 += STEP) {
+                constexpr int DU = 32 * C::ROW / 16;  // chunks from dG's tile to dU's
+                for (int c0 = 0; c0 < BN / 4; c0 += STEP) {
                     uint32_t g[STEP], u[STEP];
+                    const uint32_t at = acc + uint32_t(part * (BN / 4) + c0);
                     if constexpr (STEP == 32) {
-                        tmem_ld32(acc + uint32_t(c0), g);
-                        tmem_ld32(acc + uint32_t(BN / 2 + c0), u);
+                        tmem_ld32(at, g);
+                        tmem_ld32(at + BN / 2, u);
                     } else {
-                        tmem_ld16(acc + uint32_t(c0), g);
-                        tmem_ld16(acc + uint32_t(BN / 2 + c0), u);
+                        tmem_ld16(at, g);
+                        tmem_ld16(at + BN / 2, u);
                     }
                     tmem_wait_ld();
                     reg_fence(g), reg_fence(u);
-                    const int col = t.col0 + c0;
-                    if (row >= p.n) continue;
+                    if (c0 + STEP == BN / 4) release();
 #pragma unroll
                     for (int j = 0; j < STEP / 8; ++j) {
-                        if (col + 8 * j >= p.m) break;
+                        uint4 *place = chunk(lane, c0 / 8 + j);
                         uint32_t w[4];
                         if constexpr (MODE == GLU_FORWARD) {
 #pragma unroll
@@ -351,13 +423,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
                                 w[e] = pack2<T>(glu_act<ACT>(__uint_as_float(g[z])) * __uint_as_float(u[z]),
                                                 glu_act<ACT>(__uint_as_float(g[z + 1])) * __uint_as_float(u[z + 1]));
                             }
-                            T *dst = static_cast<T *>(p.out[0]) + row * p.out_stride[0] + col;
-                            reinterpret_cast<uint4 *>(dst)[j] = make_uint4(w[0], w[1], w[2], w[3]);
                         } else {
-                            Pack<T, 8> d;
-                            d.load(static_cast<const T *>(p.dout) + row * p.dout_stride + col + 8 * j);
-                            float dh[8];
-                            d.get(dh);
+                            float2 d[4];
+                            unpack2(*place, d, T());
                             uint32_t v[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -365,21 +433,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
                                 float a0, a1;
                                 const float d0 = glu_act_grad<ACT>(__uint_as_float(g[z]), &a0);
                                 const float d1 = glu_act_grad<ACT>(__uint_as_float(g[z + 1]), &a1);
-                                w[e] = pack2<T>(dh[2 * e] * __uint_as_float(u[z]) * d0,
-                                                dh[2 * e + 1] * __uint_as_float(u[z + 1]) * d1);
-                                v[e] = pack2<T>(dh[2 * e] * a0, dh[2 * e + 1] * a1);
+                                w[e] = pack2<T>(d[e].x * __uint_as_float(u[z]) * d0, d[e].y * __uint_as_float(u[z + 1]) * d1);
+                                v[e] = pack2<T>(d[e].x * a0, d[e].y * a1);
                             }
-                            const long long at = row * p.out_stride[0] + col;
-                            reinterpret_cast<uint4 *>(static_cast<T *>(p.out[0]) + at)[j] = make_uint4(w[0], w[1], w[2], w[3]);
-                            reinterpret_cast<uint4 *>(static_cast<T *>(p.out[1]) + at)[j] = make_uint4(v[0], v[1], v[2], v[3]);
+                            place[DU] = make_uint4(v[0], v[1], v[2], v[3]);
                         }
+                        *place = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
+                __syncwarp();
+                const int col = t.col0 + part * (BN / 4) + ccol * 8;
+#pragma unroll
+                for (int c = 0; c < C::CHUNKS; ++c) {
+                    const int r = row0 + c * PER + crow;
+                    if (r >= p.n || col >= p.m) continue;
+                    const uint4 *place = chunk(c * PER + crow, ccol);
+                    const long long at = r * p.out_stride[0] + col;
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.out[0]) + at) = *place;
+                    if (MODE == GLU_DGRAD) *reinterpret_cast<uint4 *>(static_cast<T *>(p.out[1]) + at) = place[DU];
+                }
+                __syncwarp();
             }
-            // The accumulator is free for the tile after next once both CTAs' warps have read it.
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive_cluster(cluster_addr(0, &accempty[buf]));
         }
     }
     // Both CTAs' barriers and shared memory stay until neither uses the other's.
@@ -390,6 +464,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<BN>::THREADS,
     if (warp == 1) tmem_dealloc_pair(tmem, 512);
     __syncwarp();
     cluster_sync_all();
+}
+
+// dx from its parts, added in order and rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256) glu_add_kernel(T *__restrict__ dx, long long stride, const float *__restrict__ parts,
+                                                      int splits, int n, int k) {
+    pdl_wait();
+    pdl_trigger();
+    const int per_row = k / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)n * per_row) return;
+    const int row = int(i / per_row), col = int(i - (long long)row * per_row) * 8;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+        Pack<float, 8> x;
+        float g[8];
+        x.load(parts + ((long long)s * n + row) * k + col);
+        x.get(g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += g[e];
+    }
+    Pack<T, 8> y;
+    y.set(f);
+    y.store(dx + row * stride + col);
 }
 
 // A few rows (single tokens in serving): the weights' bytes are what there is to

@@ -1,6 +1,8 @@
 // Launchers and C entry points (include/eg2_ops.h, part 3) of the gated
 // feed-forward projection.  Included once, at the end of kernels.cu.
 #pragma once
+#include <climits>
+
 #include "glu.cuh"
 
 namespace eg2 {
@@ -29,24 +31,47 @@ static cudaError_t glu_dispatch(unsigned type, unsigned act, F f) {
     return cudaErrorInvalidValue;
 }
 template <int MODE, int BN, typename T, int ACT>
-static cudaError_t glu_go(const GluMaps &maps, const GluParams &p, cudaStream_t s) {
+static cudaError_t glu_go(const GluMaps &maps, const GluParams &p, int clusters, cudaStream_t s) {
     static AllowSmem allow;
-    if (cudaError_t e = allow(glu_kernel<MODE, BN, T, ACT>, int(GluCfg<BN>::SMEM))) return e;
-    const int pairs = sm_count() / 2;
-    return launch_pdl(glu_kernel<MODE, BN, T, ACT>, dim3(2 * (p.tiles < pairs ? p.tiles : pairs)),
-                      dim3(GluCfg<BN>::THREADS), GluCfg<BN>::SMEM, s, maps, p);
+    if (cudaError_t e = allow(glu_kernel<MODE, BN, T, ACT>, int(GluCfg<MODE, BN>::SMEM))) return e;
+    return launch_pdl(glu_kernel<MODE, BN, T, ACT>, dim3(2 * clusters), dim3(GluCfg<MODE, BN>::THREADS), GluCfg<MODE, BN>::SMEM, s,
+                      maps, p);
 }
-// The widest tile that still gives every pair of SMs one, by the time of the
-// slowest pair: a 128-column step costs about 0.6 of a 256-column one, a
-// 64-column step 0.5.
-static int glu_pick_bn(const int tiles[3]) {
-    static const int cost[3] = {50, 60, 100};
-    const int pairs = sm_count() / 2;
-    int best = 2;
-    for (int i = 1; i >= 0; --i)
-        if (tiles[i] && ceil_div(tiles[i], pairs) * cost[i] < ceil_div(tiles[best], pairs) * cost[best]) best = i;
-    return 64 << best;
+// What the choices below weigh, in hundredths of a K step of 64 with a 256-column
+// tile (about 0.3 us): a step with tiles of 64, 128 and 256 columns (the tensor
+// cores take nearly as long for the narrow ones), and a tile's epilogue, which
+// runs under the next tile's steps but for the last one's.
+constexpr int GLU_STEP_COST[3] = {85, 90, 100}, GLU_EPI_COST[3] = {180, 350, 700};
+static long long glu_cost(long long tiles, int steps, int width, int clusters) {
+    const long long step = (long long)steps * GLU_STEP_COST[width], epi = GLU_EPI_COST[width];
+    return tiles ? (tiles + clusters - 1) / clusters * (step > epi ? step : epi) + epi : 0;
 }
+// The backward products' plan: dx's K in `splits` parts, and `dxc` clusters for
+// dx, so that the slowest cluster is done first.  Parts cost a launch that adds them.
+struct GluPlan {
+    int splits, dxc;
+};
+constexpr int GLU_PAIRS = 74;  // what workspaces are sized for
+static GluPlan glu_plan(unsigned n, unsigned k, unsigned m, bool dx, int weights, int pairs) {
+    const long long td = dx ? glu_tiles(n, k, 256) : 0, tw = weights * (long long)glu_tiles(m, k, 256);
+    const int sd = 2 * ceil_div(m, 64), sw = ceil_div(n, 64);
+    GluPlan best{1, 0};
+    long long least = LLONG_MAX;
+    for (int splits = 1; splits <= (dx ? 8 : 1) && splits <= sd; splits *= 2)
+        for (int d = td ? 1 : 0; d <= (!td ? 0 : tw ? pairs - 1 : pairs); ++d) {
+            const long long cd = td ? glu_cost(td * splits, ceil_div(sd, splits), 2, d) : 0;
+            const long long cw = tw ? glu_cost(tw, sw, 2, pairs - d) : 0;
+            // Parts: a launch to add them (1000), and their floats written and read, 18000 bytes in a unit.
+            const long long add = splits > 1 ? 1000 + (long long)n * k * (8 * splits + 2) / 18000 : 0;
+            const long long c = (cd > cw ? cd : cw) + add;
+            if (c < least) least = c, best = {splits, d};
+        }
+    return best;
+}
+// Workspace: dG and dU, then dx's parts.  A row of dG is 64 elements longer than
+// its columns where those are a multiple of 512, whose pitch keeps hitting the same L2 slices.
+static unsigned glu_pitch(unsigned m) { return m % 512 ? m : m + 64; }
+static uint64_t glu_half(unsigned n, unsigned m) { return (uint64_t(n) * glu_pitch(m) * 2 + 255) / 256 * 256; }
 
 static cudaError_t glu_check(unsigned n, unsigned k, unsigned m, unsigned type, unsigned act) {
     if ((type != EG_F16 && type != EG_BF16) || act > 1 || !k || !m || k % 8 || m % 8 || n > 0x7fffff00u ||
@@ -59,9 +84,14 @@ template <int MODE>
 static cudaError_t glu_project(const void *x, int64_t xs, const void *wg, int64_t wgs, const void *wu, int64_t wus,
                                unsigned type, unsigned act, GluParams &p, cudaStream_t s) {
     GluMaps maps{};
-    int tiles[3];
-    for (int i = 0; i < 3; ++i) tiles[i] = glu_tiles(unsigned(p.n), unsigned(p.m), 32 << i);
-    const int bn = glu_pick_bn(tiles);
+    // The width whose slowest cluster is done first; the wider one where they tie.
+    const int pairs = sm_count() / 2, steps = ceil_div(p.k, 64);
+    int bn = 256;
+    long long best = LLONG_MAX;
+    for (int i = 2; i >= 0; --i) {
+        const long long c = glu_cost(glu_tiles(unsigned(p.n), unsigned(p.m), 32 << i), steps, i, pairs);
+        if (c < best) best = c, bn = 64 << i;
+    }
     const unsigned wrows = bn == 64 ? 32 : 64;
     if (!glu_tmap(&maps.x, type, x, xs, unsigned(p.k), unsigned(p.n), 64) ||
         !glu_tmap(&maps.wg, type, wg, wgs, unsigned(p.k), unsigned(p.m), wrows) ||
@@ -69,12 +99,13 @@ static cudaError_t glu_project(const void *x, int64_t xs, const void *wg, int64_
         return cudaErrorInvalidValue;
     p.tiles = glu_tiles(unsigned(p.n), unsigned(p.m), bn / 2);
     p.group = 8;
+    const int clusters = p.tiles < pairs ? p.tiles : pairs;
     return glu_dispatch(type, act, [&](auto t, auto a) {
         using T = typename decltype(t)::type;
         constexpr int ACT = decltype(a)::value;
-        if (bn == 256) return glu_go<MODE, 256, T, ACT>(maps, p, s);
-        if (bn == 128) return glu_go<MODE, 128, T, ACT>(maps, p, s);
-        return glu_go<MODE, 64, T, ACT>(maps, p, s);
+        if (bn == 256) return glu_go<MODE, 256, T, ACT>(maps, p, clusters, s);
+        if (bn == 128) return glu_go<MODE, 128, T, ACT>(maps, p, clusters, s);
+        return glu_go<MODE, 64, T, ACT>(maps, p, clusters, s);
     });
 }
 
@@ -134,31 +165,37 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
     if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255) ||
         a.workspace_bytes < eg2_glu_grad_workspace(a.n, a.k, a.m))
         return cudaErrorInvalidValue;
-    uint8_t *dg = static_cast<uint8_t *>(a.workspace), *du = dg + eg2_glu_grad_workspace(a.n, a.k, a.m) / 2;
+    uint8_t *dg = static_cast<uint8_t *>(a.workspace), *du = dg + glu_half(a.n, a.m);
     GluParams p{};
     p.n = int(a.n), p.k = int(a.k), p.m = int(a.m);
     p.dout = a.dout, p.dout_stride = os;
-    p.out[0] = dg, p.out[1] = du, p.out_stride[0] = p.out_stride[1] = a.m;
+    p.out[0] = dg, p.out[1] = du, p.out_stride[0] = p.out_stride[1] = glu_pitch(a.m);
     if (cudaError_t e = glu_project<GLU_DGRAD>(a.x, xs, a.w_gate, gs, a.w_up, us, a.type, a.act, p, s)) return e;
 
     GluMaps maps{};
     if (!glu_tmap(&maps.x, a.type, a.x, xs, a.k, a.n, 64) || !glu_tmap(&maps.wg, a.type, a.w_gate, gs, a.k, a.m, 64) ||
-        !glu_tmap(&maps.wu, a.type, a.w_up, us, a.k, a.m, 64) || !glu_tmap(&maps.dg, a.type, dg, a.m, a.m, a.n, 64) ||
-        !glu_tmap(&maps.du, a.type, du, a.m, a.m, a.n, 64))
+        !glu_tmap(&maps.wu, a.type, a.w_up, us, a.k, a.m, 64) || !glu_tmap(&maps.dg, a.type, dg, glu_pitch(a.m), a.m, a.n, 64) ||
+        !glu_tmap(&maps.du, a.type, du, glu_pitch(a.m), a.m, a.n, 64))
         return cudaErrorInvalidValue;
     p.out[0] = a.dx, p.out[1] = a.dw_gate, p.out[2] = a.dw_up;
     p.out_stride[0] = dxs, p.out_stride[1] = dgs, p.out_stride[2] = dus;
     p.dw_f32 = a.dw_type == EG_F32, p.dw_accumulate = a.accumulate != 0;
-    const int weights = (a.dw_gate != nullptr) + (a.dw_up != nullptr);
-    auto count = [&](int bn) { return (a.dx ? glu_tiles(a.n, a.k, bn) : 0) + weights * glu_tiles(a.m, a.k, bn); };
-    const int tiles[3] = {0, count(128), count(256)};
-    const int bn = glu_pick_bn(tiles);
-    p.dx_tiles = a.dx ? glu_tiles(a.n, a.k, bn) : 0;
-    p.tiles = count(bn);
+    const int weights = (a.dw_gate != nullptr) + (a.dw_up != nullptr), pairs = sm_count() / 2;
+    const GluPlan plan = glu_plan(a.n, a.k, a.m, a.dx != nullptr, weights, pairs < GLU_PAIRS ? pairs : GLU_PAIRS);
+    const int w_tiles = weights * glu_tiles(a.m, a.k, 256);
+    p.splits = plan.splits, p.parts = reinterpret_cast<float *>(dg + 2 * glu_half(a.n, a.m));
+    p.dx_tiles = a.dx ? glu_tiles(a.n, a.k, 256) * plan.splits : 0;
+    p.tiles = p.dx_tiles + w_tiles;
+    p.dx_clusters = plan.dxc < p.dx_tiles ? plan.dxc : p.dx_tiles;
+    const int clusters = p.dx_clusters + (w_tiles < pairs - plan.dxc ? w_tiles : pairs - plan.dxc);
     p.group = 8;
     return glu_dispatch(a.type, 0, [&](auto t, auto) {
         using T = typename decltype(t)::type;
-        return bn == 256 ? glu_go<GLU_PRODUCTS, 256, T, 0>(maps, p, s) : glu_go<GLU_PRODUCTS, 128, T, 0>(maps, p, s);
+        if (cudaError_t e = glu_go<GLU_PRODUCTS, 256, T, 0>(maps, p, clusters, s)) return e;
+        if (!a.dx || p.splits < 2) return cudaSuccess;
+        return launch_pdl(glu_add_kernel<T>, dim3(ceil_div((long long)a.n * (a.k / 8), 256)), dim3(256), 0, s,
+                          static_cast<T *>(a.dx), (long long)dxs, static_cast<const float *>(p.parts), p.splits,
+                          p.n, p.k);
     });
 }
 
@@ -167,8 +204,13 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
 extern "C" {
 int eg2_launch_glu(const EgGlu *p, void *s) { return rc(glu(*p, S(s))); }
 uint64_t eg2_glu_grad_workspace(unsigned n, unsigned k, unsigned m) {
-    (void)k;
-    return 2 * ((uint64_t(n) * m * 2 + 255) / 256 * 256);
+    if (!n || !k || !m) return 0;
+    int splits = 1;  // the most that dx, alone or beside one or both weights' gradients, may take
+    for (int w = 0; w <= 2; ++w) {
+        const int s = glu_plan(n, k, m, true, w, GLU_PAIRS).splits;
+        if (s > splits) splits = s;
+    }
+    return 2 * glu_half(n, m) + (splits > 1 ? uint64_t(splits) * n * k * 4 : 0);
 }
 int eg2_launch_glu_grad(const EgGluGrad *p, void *s) { return rc(glu_grad(*p, S(s))); }
 }
