@@ -200,11 +200,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<MODE, BN>::TH
         fence_bar_init();
     }
     if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
-    pdl_wait();
-    pdl_trigger();
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
+    pdl_wait();
+    pdl_trigger();
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {

@@ -57,8 +57,13 @@ static GluPlan glu_plan(unsigned n, unsigned k, unsigned m, bool dx, int weights
     const int sd = 2 * ceil_div(m, 64), sw = ceil_div(n, 64);
     GluPlan best{1, 0};
     long long least = LLONG_MAX;
+    // Clusters for dx: near its share of the steps.
+    const long long steps_d = td * sd, steps_w = tw * sw;
+    const int low = td ? 1 : 0, high = !td ? 0 : tw ? pairs - 1 : pairs;
+    const int near = steps_d + steps_w ? int(pairs * steps_d / (steps_d + steps_w)) : 0;
     for (int splits = 1; splits <= (dx ? 8 : 1) && splits <= sd; splits *= 2)
-        for (int d = td ? 1 : 0; d <= (!td ? 0 : tw ? pairs - 1 : pairs); ++d) {
+        for (int off = -4; off <= 4; ++off) {
+            const int d = near + off < low ? low : near + off > high ? high : near + off;
             const long long cd = td ? glu_cost(td * splits, ceil_div(sd, splits), 2, d) : 0;
             const long long cw = tw ? glu_cost(tw, sw, 2, pairs - d) : 0;
             // Parts: a launch to add them (1000), and their floats written and read, 18000 bytes in a unit.

@@ -46,6 +46,12 @@ struct AllowSmem {
     }
 };
 
+// Whether vectors of `bytes` bytes (of `size`-byte elements) fit every one of `rows` rows at p.
+static bool rows_fit(const void *p, long long stride, unsigned rows, int bytes, int size) {
+    const int w = bytes < 16 ? bytes : 16;
+    return reinterpret_cast<uintptr_t>(p) % w == 0 && (rows < 2 || stride * size % w == 0);
+}
+
 // ---------------------------------------------------------------- embed_rows
 static cudaError_t embed_rows(const EgEmbedRows &a, cudaStream_t s) {
     const int so = type_size(a.out_type), st = type_size(a.table_type);
@@ -57,20 +63,18 @@ static cudaError_t embed_rows(const EgEmbedRows &a, cudaStream_t s) {
         return cudaErrorInvalidValue;
     const EmbedRowsParams p{a.out, a.table, a.ids, a.out_stride, a.table_stride, int(a.n), int(a.vocab), int(a.d),
                             a.scale};
-    const bool wide = a.d % 8 == 0 && aligned16(a.out) && aligned16(a.table) &&
-                      (a.n == 1 || a.out_stride * so % 16 == 0) && (a.vocab < 2 || a.table_stride * st % 16 == 0);
     return by_type(a.table_type, [&](auto ti) {
         return by_type(a.out_type, [&](auto to) {
             using TI = typename decltype(ti)::type;
             using TO = typename decltype(to)::type;
-            // Four rows a warp while that still fills the GPU, else one.
-            const bool four = a.n >= 16384;
-            const dim3 grid(ceil_div(a.n, four ? 32 : 8));
-            if (wide)
-                return four ? launch_pdl(embed_rows_kernel<TI, TO, 8, 4>, grid, dim3(256), 0, s, p)
-                            : launch_pdl(embed_rows_kernel<TI, TO, 8, 1>, grid, dim3(256), 0, s, p);
-            return four ? launch_pdl(embed_rows_kernel<TI, TO, 1, 4>, grid, dim3(256), 0, s, p)
-                        : launch_pdl(embed_rows_kernel<TI, TO, 1, 1>, grid, dim3(256), 0, s, p);
+            const auto fit = [&](int v) {
+                return a.d % v == 0 && rows_fit(a.out, a.out_stride, a.n, v * so, so) &&
+                       rows_fit(a.table, a.table_stride, a.vocab, v * st, st);
+            };
+            const dim3 grid(ceil_div(a.n, 8));
+            if (fit(8)) return launch_pdl(embed_rows_kernel<TI, TO, 8>, grid, dim3(256), 0, s, p);
+            if (fit(2)) return launch_pdl(embed_rows_kernel<TI, TO, 2>, grid, dim3(256), 0, s, p);
+            return launch_pdl(embed_rows_kernel<TI, TO, 1>, grid, dim3(256), 0, s, p);
         });
     });
 }
@@ -184,12 +188,9 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
     u.scale = a.scale, u.accumulate = a.accumulate != 0;
     u.fill = share(-1, EmbedSum::WARPS, true);
     // 16 bytes of dout per lane and row where all rows allow it, else pairs, else single elements.
-    const auto rows_fit = [&](int v) {
-        auto fits = [&](const void *p, long long row_stride, unsigned rows, int bytes) {
-            const int w = bytes < 16 ? bytes : 16;
-            return reinterpret_cast<uintptr_t>(p) % w == 0 && (rows < 2 || row_stride * (bytes / v) % w == 0);
-        };
-        return a.d % v == 0 && fits(a.dout, a.dout_stride, a.n, v * sg) && fits(a.dtable, stride, a.vocab, v * sw);
+    const auto fit = [&](int v) {
+        return a.d % v == 0 && rows_fit(a.dout, a.dout_stride, a.n, v * sg, sg) &&
+               rows_fit(a.dtable, stride, a.vocab, v * sw, sw);
     };
     return by_type(a.dout_type, [&](auto tg) {
         return by_type(a.dtable_type, [&](auto tw) {
@@ -207,7 +208,7 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
                 return launch_pdl(embed_join_kernel<TW, V>, dim3(ceil_div(L.chunks, 32), u.col_blocks), dim3(256), 0, s, u);
             };
             constexpr int WIDE = 16 / int(sizeof(TG));
-            return rows_fit(WIDE) ? go(Int<WIDE>{}) : rows_fit(2) ? go(Int<2>{}) : go(Int<1>{});
+            return fit(WIDE) ? go(Int<WIDE>{}) : fit(2) ? go(Int<2>{}) : go(Int<1>{});
         });
     });
 }
@@ -324,6 +325,7 @@ static cudaError_t qkv_norm_rope(const EgQkvNormRope &a, cudaStream_t s) {
         return e;
     const long long rows = (long long)p.n * (p.part[0].heads + p.part[1].heads + p.part[2].heads);
     if (!rows) return cudaSuccess;
+    if (rows >> 33) return cudaErrorInvalidValue;  // at least 8 rows a CTA: fewer than 2^31 CTAs
     return by_type(a.type, [&](auto t) {
         using T = typename decltype(t)::type;
         return qkv_shape<T>(p.d / 2, wide, [&](auto v, auto g, auto nv) {

@@ -198,15 +198,15 @@ def _lead(t, name, dims):
 def _check(t, name, shape, device, dtype):
     """The strides of a tensor of that shape, device and type whose last dimension is contiguous."""
     stride = t.stride()
+    if t.dtype is dtype and t.shape == shape and t.device == device and (stride[-1] == 1 or shape[-1] < 2):
+        return stride
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: expected {tuple(shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}: expected {device}")
     if t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}: expected {dtype}")
-    if stride[-1] != 1 and shape[-1] > 1:
-        raise ValueError(f"{name}'s rows are not contiguous (last stride {stride[-1]})")
-    return stride
+    raise ValueError(f"{name}'s rows are not contiguous (last stride {stride[-1]})")
 
 
 def _rows(t, name, width, device):
@@ -266,7 +266,8 @@ def embed_rows_grad(dtable, dout, ids, scale=1.0, accumulate=False, workspace=No
 
 def _qkv_args(x, q_weight, k_weight, rope_cos, rope_sin, pos):
     """Sizes and types; the first given of queries, keys and values sets n, d, device and type."""
-    lead = x[0] if x[0] is not None else x[1] if x[1] is not None else x[2]
+    q, k, v = x
+    lead = q if q is not None else k if k is not None else v
     if lead is None:
         raise ValueError("queries, keys and values are all None")
     (n, _, d), dev, _ = _lead(lead, "x", 3)
@@ -284,12 +285,16 @@ def _qkv_args(x, q_weight, k_weight, rope_cos, rope_sin, pos):
         _check(q_weight, "q_weight", (d,), dev, wdtype)
     if k_weight is not None:
         _check(k_weight, "k_weight", (d,), dev, wdtype)
-    positions, cos_stride = _rows(rope_cos, "rope_cos", d // 2, dev)
-    sin_stride = _check(rope_sin, "rope_sin", rope_cos.shape, dev, torch.float32)[0]
-    if rope_cos.dtype != torch.float32 or (positions > 1 and not cos_stride == sin_stride == d // 2):
-        raise ValueError("rope_cos and rope_sin must be contiguous float32")
+    half = d // 2
+    table = rope_cos.shape
+    if len(table) != 2 or table[1] != half:
+        raise ValueError(f"rope_cos has shape {tuple(table)}: expected (any, {half})")
+    cos_stride = _check(rope_cos, "rope_cos", table, dev, torch.float32)[0]
+    sin_stride = _check(rope_sin, "rope_sin", table, dev, torch.float32)[0]
+    if table[0] > 1 and not cos_stride == sin_stride == half:
+        raise ValueError("rope_cos and rope_sin must be contiguous")
     heads = [0 if t is None else t.shape[1] if t.dim() == 3 else -1 for t in x]
-    return (n, *heads, d, positions, code, wtype), dev, dtype
+    return (n, *heads, d, table[0], code, wtype), dev, dtype
 
 
 def _qkv_tensors(names, tensors, sizes, dev, dtype):
@@ -302,9 +307,12 @@ def _qkv_tensors(names, tensors, sizes, dev, dtype):
                 raise ValueError(f"{names[i]} is None: expected {heads} heads")
             ptrs.append(0)
             strides += (0, 0)
-        else:
-            strides += _check(t, names[i], (n, heads, d), dev, dtype)[:2]
-            ptrs.append(t.data_ptr())
+            continue
+        stride = t.stride()
+        if t.dtype is not dtype or t.shape != (n, heads, d) or t.device != dev or stride[2] != 1:
+            _check(t, names[i], (n, heads, d), dev, dtype)  # raises, saying what is wrong
+        ptrs.append(t.data_ptr())
+        strides += stride[:2]
     return ptrs, strides
 
 
