@@ -79,15 +79,14 @@ struct EmbedFill {
     const unsigned char *touched;  // null: all rows of the share
     long long stride, block0, blocks;
     int width, rows;               // bytes of a row; rows of the table
-    int ctas, per_warp;            // a CTA's warps take per_warp blocks each, so that the CTAs stay short
+    int ctas, each;                // a CTA clears `each` consecutive blocks, a warp one at a time
 };
 __device__ __forceinline__ void embed_fill(const EmbedFill &f, int cta) {
     const uint4 z = make_uint4(0, 0, 0, 0);
     const int lane = threadIdx.x & 31;
     const bool wide = ((reinterpret_cast<uintptr_t>(f.table) | uintptr_t(f.stride) | unsigned(f.width)) & 15) == 0;
-    const int warps = blockDim.x >> 5;
-    long long i = (long long)cta * warps * f.per_warp + (threadIdx.x >> 5);
-    for (int n = 0; n < f.per_warp && i < f.blocks; ++n, i += warps) {
+    const long long end = min(f.blocks, (cta + 1ll) * f.each);
+    for (long long i = (long long)cta * f.each + (threadIdx.x >> 5); i < end; i += blockDim.x >> 5) {
         const long long row0 = (f.block0 + i) * 8;
         const int rows = int(min(8ll, f.rows - row0));
         const unsigned skip =
@@ -269,13 +268,13 @@ __global__ void __launch_bounds__(EmbedSort::THREADS) embed_scatter_kernel(const
     }
 }
 
-// The same sort of up to 8192 items by one CTA in one launch: the items stay in
-// registers, up to 8 a thread, and change places through shared memory; the last
+// The same sort of up to 4096 items by one CTA in one launch: the items stay in
+// registers, up to 4 a thread, and change places through shared memory; the last
 // pass writes to memory.  The other CTAs clear the table meanwhile.  (Clusters of 8
 // and 16 CTAs that sort up to 131072 items this way, through distributed shared
 // memory, took longer than the launches above: 65 and 41 us against 36 at 100003.)
 struct EmbedSmall {
-    static constexpr int THREADS = 1024, WARPS = 32, MAX_PER = 8, CAP = THREADS * MAX_PER;
+    static constexpr int THREADS = 1024, WARPS = 32, MAX_PER = 4, CAP = THREADS * MAX_PER;
     static constexpr int BINS = EmbedSort::MAX_BINS;
     static constexpr int SMEM = CAP * 8 + WARPS * BINS * 2 + BINS * 4 + WARPS * 4;
 };
@@ -405,21 +404,24 @@ struct EmbedSumParams {
     EmbedFill fill;
 };
 template <typename TW, int V>
-__device__ __forceinline__ void embed_write_row(const EmbedSumParams &p, unsigned id, int c, const float (&acc)[V]) {
-    TW *dst = static_cast<TW *>(p.dtable) + (long long)id * p.dtable_stride + c;
-    float f[V];
+__device__ __forceinline__ TW *embed_row(const EmbedSumParams &p, unsigned id, int c) {
+    return static_cast<TW *>(p.dtable) + (long long)id * p.dtable_stride + c;
+}
+// scale * acc, added to what the row held (read before) when accumulating, rounded once.
+template <typename TW, int V>
+__device__ __forceinline__ void embed_write_row(const EmbedSumParams &p, unsigned id, int c, const float (&acc)[V],
+                                                const Pack<TW, V> &held) {
+    float f[V], old[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = acc[i] * p.scale;
-    Pack<TW, V> y;
     if (p.accumulate) {
-        float old[V];
-        y.load(dst);
-        y.get(old);
+        held.get(old);
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] += old[i];
     }
+    Pack<TW, V> y;
     y.set(f);
-    y.store(dst);
+    y.store(embed_row<TW, V>(p, id, c));
 }
 // Rows of whole 16-byte vectors (V of them a lane) come through a ring in shared
 // memory, by cp.async, two units of 8 rows ahead of the one being added; each lane
@@ -492,6 +494,14 @@ __global__ void __launch_bounds__(EmbedSum::THREADS) embed_sum_kernel(const __gr
         for (int j = 0; j < 4; ++j) {
             if (u0 + j >= units) break;
             Pack<TG, V> x[E::UNIT];
+            Pack<TW, V> held[E::UNIT];  // accumulating: the rows that end here, asked for together
+#pragma unroll
+            for (int r = 0; r < E::UNIT; ++r) {
+                held[r].zero();
+                if (!p.accumulate || !(ends >> (j * 8 + r) & 1)) continue;
+                const unsigned id = __shfl_sync(0xffffffffu, now.x, j * 8 + r);
+                if (mine) held[r].load(embed_row<TW, V>(p, id, c));
+            }
             if constexpr (STREAM) {
                 const int to = stage == 0 ? 2 : stage - 1;  // (stage + 2) % 3
                 if (u0 + j + 2 < units) fetch(to, j < 2 ? now : then, ((j + 2) & 3) * 8);
@@ -522,7 +532,7 @@ __global__ void __launch_bounds__(EmbedSum::THREADS) embed_sum_kernel(const __gr
                     sum.set(acc);
                     if (from_before) sum.store(p.head + (size_t)ch * p.d + c);
                     else if (base + j * 8 + r == i1 - 1 && id == next) sum.store(p.tail + (size_t)ch * p.d + c);
-                    else embed_write_row<TW, V>(p, id, c, acc);
+                    else embed_write_row<TW, V>(p, id, c, acc, held[r]);
                 }
                 from_before = false;
 #pragma unroll
@@ -587,6 +597,9 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const __grid_constant__
         } else if (mine) {
             float acc[V];
             Pack<float, V> x;
+            Pack<TW, V> held;
+            held.zero();
+            if (p.accumulate) held.load(embed_row<TW, V>(p, run, c));
             x.load(p.tail + (size_t)first * p.d + c);
             x.get(acc);
 #pragma unroll 4
@@ -597,7 +610,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[i] += f[i];
             }
-            embed_write_row<TW, V>(p, p.items[(long long)(first + 1) * p.chunk].x, c, acc);
+            embed_write_row<TW, V>(p, run, c, acc, held);
         }
     }
     __syncthreads();
@@ -626,13 +639,17 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const __grid_constant__
         for (int i = 0; i < V; ++i) part[warp][lane * V + i] = acc[i];
         __syncthreads();
         if (warp == 0 && mine) {
+            const unsigned run = p.items[(long long)(first + 1) * p.chunk].x;
+            Pack<TW, V> held;
+            held.zero();
+            if (p.accumulate) held.load(embed_row<TW, V>(p, run, c));
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] = 0.0f;
             for (int w = 0; w < 8; ++w) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[i] += part[w][lane * V + i];
             }
-            embed_write_row<TW, V>(p, p.items[(long long)(first + 1) * p.chunk].x, c, acc);
+            embed_write_row<TW, V>(p, run, c, acc, held);
         }
         __syncthreads();
     }

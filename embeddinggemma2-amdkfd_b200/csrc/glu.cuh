@@ -493,43 +493,56 @@ __global__ void __launch_bounds__(256) glu_add_kernel(T *__restrict__ dx, long l
 }
 
 // A few rows (single tokens in serving): the weights' bytes are what there is to
-// move, and the tensor cores' 256-row tiles would be empty.  A warp takes one
-// output column: both weight rows stream through registers once, against up to NT rows of x.
-template <typename T, int ACT, int NT>
+// move, and the tensor cores' 256-row tiles would be empty.  A warp takes COLS
+// output columns: their weight rows stream through registers once, against NT
+// rows of x, each of whose vectors serves all COLS columns.
+template <typename T, int ACT, int NT, int COLS>
 __global__ void __launch_bounds__(256) glu_rows_kernel(T *__restrict__ out, long long out_stride,
                                                        const T *__restrict__ x, long long x_stride,
                                                        const T *__restrict__ wg, long long wg_stride,
-                                                       const T *__restrict__ wu, long long wu_stride, int n, int k, int m) {
+                                                       const T *__restrict__ wu, long long wu_stride, int k, int m) {
     pdl_wait();
     pdl_trigger();
-    const int col = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (col >= m) return;
-    float g[NT], u[NT];
+    const int col = (blockIdx.x * 8 + (threadIdx.x >> 5)) * COLS, lane = threadIdx.x & 31;
+    if (col >= m) return;  // m is a multiple of COLS
+    float2 g[NT][COLS], u[NT][COLS];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) g[t] = u[t] = 0.0f;
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) g[t][c] = u[t][c] = make_float2(0.0f, 0.0f);
 #pragma unroll 2
-    for (int c = lane * 8; c < k; c += 256) {
-        Pack<T, 8> a, b;
-        a.load(wg + col * wg_stride + c);
-        b.load(wu + col * wu_stride + c);
-        float fa[8], fb[8];
-        a.get(fa), b.get(fb);
+    for (int i = lane * 8; i < k; i += 256) {
+        uint4 a[COLS], b[COLS], y[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (t >= n) break;
-            Pack<T, 8> y;
-            float fx[8];
-            y.load(x + t * x_stride + c);
-            y.get(fx);
+        for (int c = 0; c < COLS; ++c) {
+            a[c] = *reinterpret_cast<const uint4 *>(wg + (col + c) * wg_stride + i);
+            b[c] = *reinterpret_cast<const uint4 *>(wu + (col + c) * wu_stride + i);
+        }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[t] = fmaf(fx[e], fa[e], g[t]), u[t] = fmaf(fx[e], fb[e], u[t]);
+        for (int t = 0; t < NT; ++t) y[t] = *reinterpret_cast<const uint4 *>(x + t * x_stride + i);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            float2 fa[4], fb[4];
+            unpack2(a[c], fa, T()), unpack2(b[c], fb, T());
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float2 fx[4];
+                unpack2(y[t], fx, T());
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    g[t][c] = fma2(fx[e], fa[e], g[t][c]);
+                    u[t][c] = fma2(fx[e], fb[e], u[t][c]);
+                }
+            }
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float gs = warp_sum_f(g[t]), us = warp_sum_f(u[t]);
-        if (lane == 0 && t < n) out[t * out_stride + col] = from_f32<T>(glu_act<ACT>(gs) * us);
-    }
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            const float gs = warp_sum_f(g[t][c].x + g[t][c].y), us = warp_sum_f(u[t][c].x + u[t][c].y);
+            if (lane == 0) out[t * out_stride + col + c] = from_f32<T>(glu_act<ACT>(gs) * us);
+        }
 }
 
 }  // namespace eg2

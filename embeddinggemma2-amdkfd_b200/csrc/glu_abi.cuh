@@ -7,7 +7,9 @@
 
 namespace eg2 {
 
-constexpr unsigned GLU_FEW_ROWS = 8;  // up to this many rows run on the CUDA cores
+// Up to this many rows run on the CUDA cores: 4 rows x 2048 x 8192 take no longer
+// there than on the tensor cores (about 19 us), 8 took 34 against 20.
+constexpr unsigned GLU_FEW_ROWS = 4;
 
 // [rows][width] of a 16-bit type, boxes of 64 elements x box_rows, 128-byte swizzle.
 static bool glu_tmap(CUtensorMap *map, unsigned type, const void *base, int64_t stride, unsigned width, unsigned rows,
@@ -73,10 +75,8 @@ static GluPlan glu_plan(unsigned n, unsigned k, unsigned m, bool dx, int weights
         }
     return best;
 }
-// Workspace: dG and dU, then dx's parts.  A row of dG is 64 elements longer than
-// its columns where those are a multiple of 512, whose pitch keeps hitting the same L2 slices.
-static unsigned glu_pitch(unsigned m) { return m % 512 ? m : m + 64; }
-static uint64_t glu_half(unsigned n, unsigned m) { return (uint64_t(n) * glu_pitch(m) * 2 + 255) / 256 * 256; }
+// Workspace: dG and dU, then dx's parts.
+static uint64_t glu_half(unsigned n, unsigned m) { return (uint64_t(n) * m * 2 + 255) / 256 * 256; }
 
 static cudaError_t glu_check(unsigned n, unsigned k, unsigned m, unsigned type, unsigned act) {
     if ((type != EG_F16 && type != EG_BF16) || act > 1 || !k || !m || k % 8 || m % 8 || n > 0x7fffff00u ||
@@ -125,16 +125,18 @@ static cudaError_t glu(const EgGlu &a, cudaStream_t s) {
         return glu_dispatch(a.type, a.act, [&](auto t, auto act) {
             using T = typename decltype(t)::type;
             constexpr int ACT = decltype(act)::value;
-            const dim3 grid(ceil_div(a.m, 8));
-            auto go = [&](auto kernel) {
-                return launch_pdl(kernel, grid, dim3(256), 0, s, static_cast<T *>(a.out), (long long)os,
-                                  static_cast<const T *>(a.x), (long long)xs, static_cast<const T *>(a.w_gate),
-                                  (long long)gs, static_cast<const T *>(a.w_up), (long long)us, int(a.n), int(a.k),
-                                  int(a.m));
+            auto go = [&](auto kernel, int cols) {
+                return launch_pdl(kernel, dim3(ceil_div(a.m, 8 * cols)), dim3(256), 0, s, static_cast<T *>(a.out),
+                                  (long long)os, static_cast<const T *>(a.x), (long long)xs,
+                                  static_cast<const T *>(a.w_gate), (long long)gs, static_cast<const T *>(a.w_up),
+                                  (long long)us, int(a.k), int(a.m));
             };
-            if (a.n == 1) return go(glu_rows_kernel<T, ACT, 1>);
-            if (a.n <= 4) return go(glu_rows_kernel<T, ACT, 4>);
-            return go(glu_rows_kernel<T, ACT, 8>);
+            switch (a.n) {
+                case 1: return go(glu_rows_kernel<T, ACT, 1, 1>, 1);
+                case 2: return go(glu_rows_kernel<T, ACT, 2, 2>, 2);
+                case 3: return go(glu_rows_kernel<T, ACT, 3, 2>, 2);
+                default: return go(glu_rows_kernel<T, ACT, 4, 2>, 2);
+            }
         });
     GluParams p{};
     p.n = int(a.n), p.k = int(a.k), p.m = int(a.m);
@@ -174,13 +176,13 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
     GluParams p{};
     p.n = int(a.n), p.k = int(a.k), p.m = int(a.m);
     p.dout = a.dout, p.dout_stride = os;
-    p.out[0] = dg, p.out[1] = du, p.out_stride[0] = p.out_stride[1] = glu_pitch(a.m);
+    p.out[0] = dg, p.out[1] = du, p.out_stride[0] = p.out_stride[1] = a.m;
     if (cudaError_t e = glu_project<GLU_DGRAD>(a.x, xs, a.w_gate, gs, a.w_up, us, a.type, a.act, p, s)) return e;
 
     GluMaps maps{};
     if (!glu_tmap(&maps.x, a.type, a.x, xs, a.k, a.n, 64) || !glu_tmap(&maps.wg, a.type, a.w_gate, gs, a.k, a.m, 64) ||
-        !glu_tmap(&maps.wu, a.type, a.w_up, us, a.k, a.m, 64) || !glu_tmap(&maps.dg, a.type, dg, glu_pitch(a.m), a.m, a.n, 64) ||
-        !glu_tmap(&maps.du, a.type, du, glu_pitch(a.m), a.m, a.n, 64))
+        !glu_tmap(&maps.wu, a.type, a.w_up, us, a.k, a.m, 64) || !glu_tmap(&maps.dg, a.type, dg, a.m, a.m, a.n, 64) ||
+        !glu_tmap(&maps.du, a.type, du, a.m, a.m, a.n, 64))
         return cudaErrorInvalidValue;
     p.out[0] = a.dx, p.out[1] = a.dw_gate, p.out[2] = a.dw_up;
     p.out_stride[0] = dxs, p.out_stride[1] = dgs, p.out_stride[2] = dus;

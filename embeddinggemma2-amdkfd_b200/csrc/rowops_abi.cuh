@@ -147,8 +147,12 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
         if (count > left) count = left;
         f.table = static_cast<unsigned char *>(a.dtable), f.touched = skip ? touched : nullptr;
         f.stride = stride * sw, f.width = int(a.d) * sw, f.rows = int(a.vocab);
-        f.per_warp = block_bytes >= 16384 ? 1 : int(16384 / block_bytes);
-        f.ctas = ceil_div(count, (long long)warps * f.per_warp);
+        // Short CTAs, about 16 KB a warp, but enough of them for every SM.
+        const long long per_warp = block_bytes >= 16384 ? 1 : 16384 / block_bytes;
+        long long ctas = (count + warps * per_warp - 1) / (warps * per_warp);
+        if (ctas < sm_count()) ctas = count < sm_count() ? count : sm_count();
+        f.each = int(ctas ? (count + ctas - 1) / ctas : 0);
+        f.ctas = f.each ? ceil_div(count, f.each) : 0;
         left -= count;
         f.block0 = left, f.blocks = count;
         return f;
