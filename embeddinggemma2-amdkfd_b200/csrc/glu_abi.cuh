@@ -40,10 +40,10 @@ static cudaError_t glu_go(const GluMaps &maps, const GluParams &p, int clusters,
                       maps, p);
 }
 // What the choices below weigh, in hundredths of a K step of 64 with a 256-column
-// tile (about 0.3 us): a step with tiles of 64, 128 and 256 columns (the tensor
-// cores take nearly as long for the narrow ones), and a tile's epilogue, which
-// runs under the next tile's steps but for the last one's.
-constexpr int GLU_STEP_COST[3] = {85, 90, 100}, GLU_EPI_COST[3] = {180, 350, 700};
+// tile (measured: 0.35 us): a step with tiles of 64, 128 and 256 columns (the
+// tensor cores take nearly as long for the narrow ones), and a tile's epilogue
+// (3.1 us at 256), which runs under the next tile's steps but for the last one's.
+constexpr int GLU_STEP_COST[3] = {85, 90, 100}, GLU_EPI_COST[3] = {230, 450, 900};
 static long long glu_cost(long long tiles, int steps, int width, int clusters) {
     const long long step = (long long)steps * GLU_STEP_COST[width], epi = GLU_EPI_COST[width];
     return tiles ? (tiles + clusters - 1) / clusters * (step > epi ? step : epi) + epi : 0;
@@ -59,20 +59,22 @@ static GluPlan glu_plan(unsigned n, unsigned k, unsigned m, bool dx, int weights
     const int sd = 2 * ceil_div(m, 64), sw = ceil_div(n, 64);
     GluPlan best{1, 0};
     long long least = LLONG_MAX;
-    // Clusters for dx: near its share of the steps.
-    const long long steps_d = td * sd, steps_w = tw * sw;
     const int low = td ? 1 : 0, high = !td ? 0 : tw ? pairs - 1 : pairs;
-    const int near = steps_d + steps_w ? int(pairs * steps_d / (steps_d + steps_w)) : 0;
-    for (int splits = 1; splits <= (dx ? 8 : 1) && splits <= sd; splits *= 2)
-        for (int off = -4; off <= 4; ++off) {
-            const int d = near + off < low ? low : near + off > high ? high : near + off;
+    for (int splits = 1; splits <= (dx ? 8 : 1) && splits <= sd; splits *= 2) {
+        // Parts: a launch to add them (900), and their floats written and read, 21000 bytes in a unit.
+        const long long add = splits > 1 ? 900 + (long long)n * k * (8 * splits + 2) / 21000 : 0;
+        int at = low;
+        long long here = LLONG_MAX;
+        const auto weigh = [&](int d) {
+            if (d < low || d > high) return;
             const long long cd = td ? glu_cost(td * splits, ceil_div(sd, splits), 2, d) : 0;
-            const long long cw = tw ? glu_cost(tw, sw, 2, pairs - d) : 0;
-            // Parts: a launch to add them (1000), and their floats written and read, 18000 bytes in a unit.
-            const long long add = splits > 1 ? 1000 + (long long)n * k * (8 * splits + 2) / 18000 : 0;
-            const long long c = (cd > cw ? cd : cw) + add;
-            if (c < least) least = c, best = {splits, d};
-        }
+            const long long cw = tw ? glu_cost(tw, sw, 2, pairs - d) : 0, c = (cd > cw ? cd : cw) + add;
+            if (c < here) here = c, at = d;
+        };
+        for (int d = low; d <= high; d += 4) weigh(d);  // coarsely, then around the best
+        for (int d = at - 3, end = at + 3; d <= end; ++d) weigh(d);
+        if (here < least) least = here, best = {splits, at};
+    }
     return best;
 }
 // Workspace: dG and dU, then dx's parts.
