@@ -34,7 +34,9 @@
 // memory, warps 4..11 epilogue (lane quadrant = warp % 4, half of the columns
 // each).  Two accumulators of BN columns, so that a tile's epilogue runs under
 // the next tile's products.  Persistent; in GLU_PRODUCTS the clusters are shared out
-// between dx's tiles (K = 2 m) and the weights' (K = n) by their lengths.
+// between dx's tiles (K = 2 m) and the weights' (K = n) by their lengths, or, where
+// there are many of both, take dx's and then the weights' together, so that those
+// running at one time share more of their operands in L2.
 #pragma once
 #include "typed.cuh"
 
@@ -70,7 +72,8 @@ struct GluParams {
     int tiles, dx_tiles, group;   // tiles in all; those of dx come first; row tiles walked together
     int splits;                   // PRODUCTS: dx's K in this many parts, a tile each; above 1 they are
     float *parts;                 // written here, [splits][n][k] in fp32, for glu_add_kernel
-    int dx_clusters;              // PRODUCTS: clusters 0 .. dx_clusters - 1 take dx's tiles, the others the weights'
+    int dx_clusters;              // PRODUCTS: clusters 0 .. dx_clusters - 1 take dx's tiles, the others the
+                                  // weights'; below 0: all of them dx's and then the weights'
 };
 
 // ---------------------------------------------------------------- cluster pieces
@@ -187,7 +190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<MODE, BN>::TH
     const int rank = int(cluster_rank());
     // This cluster's tiles: first, first + step, ... below end.
     int first = blockIdx.x / 2, step = gridDim.x / 2, end = p.tiles;
-    if (MODE == GLU_PRODUCTS) {
+    if (MODE == GLU_PRODUCTS && p.dx_clusters >= 0) {
         if (first < p.dx_clusters) step = p.dx_clusters, end = p.dx_tiles;
         else first += p.dx_tiles - p.dx_clusters, step -= p.dx_clusters;
     }

@@ -111,7 +111,7 @@ static EmbedGradLayout embed_grad_layout(unsigned n, unsigned d) {
 
 static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
     const int sw = type_size(a.dtable_type), sg = type_size(a.dout_type);
-    if (!sw || !sg || !a.d || a.d > (1u << 20) || a.n > 0x7fffffffu || a.vocab > 0x7ffffffeu)
+    if (!sw || !sg || !a.d || a.d > (1u << 20) || a.n > (1u << 30) || a.vocab > 0x7ffffffeu)
         return cudaErrorInvalidValue;
     if (!a.vocab || (!a.n && a.accumulate)) return cudaSuccess;
     if (!a.dtable || (a.vocab > 1 && a.dtable_stride < (int64_t)a.d)) return cudaErrorInvalidValue;
@@ -386,7 +386,7 @@ static cudaError_t qkv_norm_rope_grad(const EgQkvNormRopeGrad &a, cudaStream_t s
 
 extern "C" {
 int eg2_launch_embed_rows(const EgEmbedRows *p, void *s) { return rc(embed_rows(*p, S(s))); }
-uint64_t eg2_embed_rows_grad_workspace(unsigned n, unsigned d) { return embed_grad_layout(n, d).total; }
+uint64_t eg2_embed_rows_grad_workspace(unsigned n, unsigned d) { return n && d ? embed_grad_layout(n, d).total : 0; }
 int eg2_launch_embed_rows_grad(const EgEmbedRowsGrad *p, void *s) { return rc(embed_rows_grad(*p, S(s))); }
 int eg2_launch_qkv_norm_rope(const EgQkvNormRope *p, void *s) { return rc(qkv_norm_rope(*p, S(s))); }
 uint64_t eg2_qkv_norm_rope_grad_workspace(unsigned n, unsigned q_heads, unsigned kv_heads, unsigned d) {

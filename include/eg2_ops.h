@@ -130,10 +130,11 @@ typedef struct {
     void *out; const void *table; const int *ids; int64_t out_stride, table_stride;
     unsigned n, vocab, d, out_type, table_type; float scale;
 } EgEmbedRows;
-/* dtable[v] = scale * sum of dout[t] over ids[t] = v (tokens in ascending order),
+/* dtable[v] = scale * sum of dout[t] over ids[t] = v (in an order that n and d fix),
  * zero for an id that does not occur; with accumulate, added to what dtable
  * holds (rows that do not occur are then not touched).  Padding's rows of dout
- * are not read.  workspace: eg2_embed_rows_grad_workspace(n, d) bytes. */
+ * are not read.  n is at most 2^30.  workspace:
+ * eg2_embed_rows_grad_workspace(n, d) bytes. */
 typedef struct {
     void *dtable; const void *dout; const int *ids; void *workspace; uint64_t workspace_bytes;
     int64_t dtable_stride, dout_stride;
@@ -144,8 +145,9 @@ typedef struct {
  * tables rope_cos, rope_sin [positions][d/2]; values have neither weight nor
  * rotation.  Index 0, 1, 2 of an array: queries, keys, values; a stride pair is
  * (token, head).  A head count of 0 leaves that tensor out; a null weight is 1.
- * A position outside [0, positions) is padding: zeros.  d even, at most 512;
- * weight_type is EG_F32 or type.  out may be x itself. */
+ * A position outside [0, positions) is padding: zeros, and x is not read.  d
+ * even, at most 512; n at most 2^30; weight_type is EG_F32 or type.  Strides are
+ * not negative; out may be x itself. */
 typedef struct {
     void *out[3]; const void *x[3]; const void *weight[2]; const float *rope_cos, *rope_sin; const int *pos;
     int64_t out_stride[3][2], x_stride[3][2];
