@@ -13,6 +13,13 @@
 // g s(g), with the logistic s(z) = 1 / (1 + exp(-z)): gelu's 0.5 (1 + tanh v) is
 // s(2 v), which keeps its relative precision where tanh is near -1.
 //
+// Measured on B200, bf16: forward 16411 x 2048 x 8192 (1.10 TFLOP) 0.83 ms, 1.33
+// PFLOP/s with the card at its power limit, tensor pipe active on 86 % of the
+// cycles; backward 8203 x 2048 x 8192 (1.65 TFLOP) 1.35 ms, pipe 76 % (projections)
+// and 86 % (products); backward of a 2048 x 512 x 2048 wave 40 us, a third of it the
+// ramps and last epilogues of its three launches.  A 64-deep step of a 256 x 256
+// tile takes 0.34 us with or without its loads, one of 256 x 128 no less.
+//
 // One kernel carries all of it.  A cluster of two CTAs (two SMs) owns one output
 // tile of 256 rows x BN columns: each CTA loads its own 128 rows of A and half of
 // B's columns, and one tcgen05.mma.cta_group::2 per 16 of K, issued by the even

@@ -142,3 +142,94 @@ def test_training_step_against_64_bits(ops):
     graph.replay()
     check()
     assert ops.read_error() == 0
+
+
+def test_two_threads_on_two_streams(ops):
+    """Calls from two host threads at once, each on its stream with workspaces of its own (allocated by the call)."""
+    import threading
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    n, v, d, m = 5000, 3000, 128, 256
+    cos, sin = rand(64, 32), rand(64, 32)
+    w = rand(64)
+    sets = []
+    for _ in range(2):
+        x = rand(n, d).bfloat16()
+        sets.append(dict(x=x, ids=torch.randint(0, v, (n,), generator=g, device=DEV, dtype=torch.int32),
+                         pos=torch.randint(0, 64, (n,), generator=g, device=DEV, dtype=torch.int32),
+                         wg=(rand(m, d) / 8).bfloat16(), wu=(rand(m, d) / 8).bfloat16(), dout=rand(n, m).bfloat16()))
+
+    def run(s):
+        dtable, dx, rot = torch.empty(v, d, device=DEV), torch.empty_like(s["x"]), torch.empty_like(s["x"]).view(n, 2, 64)
+        dwg, dwu, dw = torch.empty(m, d, device=DEV), torch.empty(m, d, device=DEV), torch.empty(64, device=DEV)
+        out, drot = torch.empty_like(s["dout"]), torch.empty_like(rot)
+        for _ in range(5):
+            ops.glu(out, s["x"], s["wg"], s["wu"], "silu")
+            ops.glu_grad(dx, dwg, dwu, s["dout"], s["x"], s["wg"], s["wu"], "silu")
+            ops.qkv_norm_rope(rot, None, None, s["x"].view(n, 2, 64), None, None, w, None, cos, sin, s["pos"])
+            ops.qkv_norm_rope_grad(drot, None, None, dw, None, dx.view(n, 2, 64), None, None, s["x"].view(n, 2, 64),
+                                   None, None, w, None, cos, sin, s["pos"])
+            ops.embed_rows_grad(dtable, drot.view(n, d), s["ids"])
+        return out, dx, dwg, dwu, rot, drot, dw, dtable
+
+    want = [run(s) for s in sets]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got[i] = run(sets[i])
+            stream.synchronize()
+        except Exception as e:  # reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+    assert ops.read_error() == 0
+
+
+def test_first_call_may_be_captured(tmp_path):
+    """A process whose first calls are made under capture: nothing in them needs an uncaptured call before."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import importlib, torch
+ops = importlib.import_module("embeddinggemma2-amdkfd_b200.ops")
+dev = "cuda:0"
+x = torch.randn(300, 64, device=dev).bfloat16()
+w = torch.randn(128, 64, device=dev).bfloat16()
+d = torch.randn(300, 128, device=dev).bfloat16()
+ids = torch.arange(300, device=dev, dtype=torch.int32) % 7
+out, dx, dw, table = torch.empty_like(d), torch.empty_like(x), torch.empty_like(w), torch.empty(7, 64, device=dev)
+q, dq, c = torch.empty(300, 1, 64, device=dev, dtype=torch.bfloat16), torch.empty(300, 1, 64, device=dev, dtype=torch.bfloat16), torch.ones(7, 32, device=dev)
+dn, n = torch.empty(64, device=dev), torch.ones(64, device=dev)
+def step():
+    ops.glu(out, x, w, w)
+    ops.glu_grad(dx, dw, None, d, x, w, w)
+    ops.qkv_norm_rope(q, None, None, x.view(300, 1, 64), None, None, n, None, c, c, ids)
+    ops.qkv_norm_rope_grad(dq, None, None, dn, None, q, None, None, x.view(300, 1, 64), None, None, n, None, c, c, ids)
+    ops.embed_rows_grad(table, dx, ids)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step()
+graph.replay()
+got = [t.clone() for t in (out, dx, dw, q, dq, dn, table)]
+step()
+assert all(torch.equal(a, b) for a, b in zip(got, (out, dx, dw, q, dq, dn, table)))
+assert ops.read_error() == 0
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
