@@ -101,7 +101,8 @@ def inputs(n, k, m, dtype, seed):
 
 
 SHAPES = [(1, 8, 8), (1, 512, 2048), (3, 200, 40), (8, 264, 72), (9, 8, 8), (9, 512, 2048), (64, 72, 264),
-          (128, 64, 64), (129, 512, 96), (257, 136, 328), (300, 1032, 520), (513, 512, 2048), (2048, 512, 2048)]
+          (128, 64, 64), (129, 512, 96), (257, 136, 328), (300, 1032, 520), (513, 512, 2048), (2048, 512, 2048), (5, 40, 8200),
+          (40, 264, 4104), (700, 2568, 136), (6000, 520, 2056), (9003, 1032, 264)]
 
 
 @pytest.mark.parametrize("n,k,m", SHAPES)

@@ -325,7 +325,13 @@ SHAPES = [(1, 4, 2, 256), (1, 1, 1, 2), (3, 4, 1, 512), (33, 3, 3, 48), (70, 5, 
           (65, 2, 1, 64), (40, 6, 2, 96), (31, 2, 2, 192), (50, 3, 1, 34), (2011, 4, 2, 256), (4099, 10, 2, 32)]
 
 
-@pytest.mark.parametrize("n,hq,hkv,d", SHAPES)
+# Rows enough for the streaming form of the forward pass in every type: whole and
+# partial halves, odd head counts, the widest rows, and more heads than groups of lanes.
+LARGE = [(9001, 2, 1, 512), (12007, 8, 2, 128), (16001, 6, 2, 96), (30011, 3, 1, 48), (9001, 5, 1, 80),
+         (21, 6000, 1, 256)]
+
+
+@pytest.mark.parametrize("n,hq,hkv,d", SHAPES + LARGE)
 @pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (F16, F16), (BF16, BF16)])
 def test_qkv_norm_rope(ops, n, hq, hkv, d, dtype, wdtype):
     q, k, v, qw, kw, cos, sin, pos, g = qkv_inputs(n, hq, hkv, d, dtype, wdtype, n + d)
@@ -378,7 +384,7 @@ def test_qkv_norm_rope_extremes(ops):
     assert (dx[3] == 0).all() and dx.isfinite().all() and dw.isfinite().all()
 
 
-@pytest.mark.parametrize("n,hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("n,hq,hkv,d", SHAPES + LARGE)
 @pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (F16, F16), (BF16, BF16)])
 def test_qkv_norm_rope_grad(ops, n, hq, hkv, d, dtype, wdtype):
     q, k, v, qw, kw, cos, sin, pos, g = qkv_inputs(n, hq, hkv, d, dtype, wdtype, 3 * n + d)
