@@ -13,7 +13,7 @@
 //
 // Measured on B200, tables of 262144 x 512: lookup of 61447 bf16 rows 15.9 us
 // (85 MB, 5.3 TB/s); gradient of 1999 fp32 rows 83 us (541 MB, the rate of a plain
-// copy), of 100003 bf16 rows 95 us (366 MB; the sort before the sums is 35 us of it).
+// copy), of 100003 bf16 rows 93 us (366 MB; the sort before the sums is 35 us of it).
 #pragma once
 #include "typed.cuh"
 

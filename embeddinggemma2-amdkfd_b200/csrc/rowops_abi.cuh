@@ -132,8 +132,9 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
     EmbedSortParams q{};
     q.hist = reinterpret_cast<unsigned *>(ws + L.hist);
     q.n = int(a.n), q.vocab = int(a.vocab), q.tiles = L.tiles, q.subtiles = L.subtiles, q.bits = bits;
-    // The table's untouched rows are cleared beside the other work: in each launch
-    // of the sort about what can be written in the time that it takes anyway, the
+    // The table's untouched rows are cleared beside the other work: beside the sort
+    // about what can be written in the time that it takes anyway (64 MB a scatter: 93
+    // us at 100003 tokens, 95 with 32 or 134 MB, 96 also beside the histograms), the
     // rest beside the sums.  A larger vocabulary than there are flags for is
     // cleared whole before the sums.
     const bool flags_fit = a.vocab <= EmbedSort::MAX_TOUCHED;
@@ -177,7 +178,7 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
             for (int half = 0; half < 2; ++half) {
                 const bool last = pass == passes - 1 && half;
                 q.touched = pass == passes - 1 ? touched : nullptr;
-                q.fill = share(last && !flags_fit ? -1 : half ? 32 << 20 : 0, EmbedSort::WARPS, false);
+                q.fill = share(last && !flags_fit ? -1 : half ? 64 << 20 : 0, EmbedSort::WARPS, false);
                 if (cudaError_t e = launch_pdl(half ? embed_scatter_kernel : embed_hist_kernel,
                                                dim3(L.tiles + q.fill.ctas), dim3(EmbedSort::THREADS), 0, s, q))
                     return e;
