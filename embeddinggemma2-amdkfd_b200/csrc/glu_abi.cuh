@@ -1,9 +1,8 @@
 // Launchers and C entry points (include/eg2_ops.h, part 3) of the gated
 // feed-forward projection.  Included once, at the end of kernels.cu.
 #pragma once
-#include <climits>
-
 #include "glu.cuh"
+#include "glu_plan.h"
 
 namespace eg2 {
 
@@ -22,7 +21,6 @@ static bool glu_matrix_ok(const void *p, int64_t *stride, unsigned width, unsign
     if (rows < 2) *stride = width;
     return p && aligned16(p) && *stride >= int64_t(width) && *stride * size % 16 == 0 && *stride < (1ll << 36);
 }
-static int glu_tiles(unsigned rows, unsigned cols, int bn) { return ceil_div(rows, 256) * ceil_div(cols, bn); }
 
 // f(type tag, activation) for the kernels' template arguments.
 template <typename F>
@@ -39,58 +37,8 @@ static cudaError_t glu_go(const GluMaps &maps, const GluParams &p, int clusters,
     return launch_pdl(glu_kernel<MODE, BN, T, ACT>, dim3(2 * clusters), dim3(GluCfg<MODE, BN>::THREADS), GluCfg<MODE, BN>::SMEM, s,
                       maps, p);
 }
-// What the choices below weigh, in hundredths of a K step of 64 with a 256-column
-// tile (measured: 0.35 us): a step with tiles of 64, 128 and 256 columns (the
-// tensor cores take nearly as long for the narrow ones), and a tile's epilogue
-// (3.1 us at 256), which runs under the next tile's steps but for the last one's.
-constexpr int GLU_STEP_COST[3] = {85, 90, 100}, GLU_EPI_COST[3] = {230, 450, 900};
-static long long glu_cost(long long tiles, int steps, int width, int clusters) {
-    const long long step = (long long)steps * GLU_STEP_COST[width], epi = GLU_EPI_COST[width];
-    return tiles ? (tiles + clusters - 1) / clusters * (step > epi ? step : epi) + epi : 0;
-}
-// The backward products' plan: dx's K in `splits` parts, and `dxc` clusters for
-// dx, so that the slowest cluster is done first.  Parts cost a launch that adds them.
-struct GluPlan {
-    int splits, dxc;  // dxc < 0: all clusters take dx's tiles and then the weights'
-};
-constexpr int GLU_PAIRS = 74;  // what workspaces are sized for
-static GluPlan glu_plan(unsigned n, unsigned k, unsigned m, bool dx, int weights, int pairs) {
-    const long long td = dx ? glu_tiles(n, k, 256) : 0, tw = weights * (long long)glu_tiles(m, k, 256);
-    const int sd = 2 * ceil_div(m, 64), sw = ceil_div(n, 64);
-    GluPlan best{1, 0};
-    long long least = LLONG_MAX;
-    const int low = td ? 1 : 0, high = !td ? 0 : tw ? pairs - 1 : pairs;
-    for (int splits = 1; splits <= (dx ? 8 : 1) && splits <= sd; splits *= 2) {
-        // Parts: a launch to add them (900), and their floats written and read, 21000 bytes in a unit.
-        const long long add = splits > 1 ? 900 + (long long)n * k * (8 * splits + 2) / 21000 : 0;
-        int at = low;
-        long long here = LLONG_MAX;
-        const auto weigh = [&](int d) {
-            if (d < low || d > high) return;
-            const long long cd = td ? glu_cost(td * splits, ceil_div(sd, splits), 2, d) : 0;
-            const long long cw = tw ? glu_cost(tw, sw, 2, pairs - d) : 0, c = (cd > cw ? cd : cw) + add;
-            if (c < here) here = c, at = d;
-        };
-        for (int d = low; d <= high; d += 4) weigh(d);  // coarsely, then around the best
-        for (int d = at - 3, end = at + 3; d <= end; ++d) weigh(d);
-        if (here < least) least = here, best = {splits, at};
-    }
-    // One after the other on all clusters, where the slowest is not later for it:
-    // 8203 x 2048 x 8192 reads 1.6 GB from memory in that order, 1.9 GB side by side.
-    if (td && tw) {
-        long long worst = 0;
-        const long long cd = glu_cost(1, sd, 2, 1) - GLU_EPI_COST[2], cw = glu_cost(1, sw, 2, 1) - GLU_EPI_COST[2];
-        for (int c = 0; c < pairs; ++c) {
-            const long long mine = (td + tw - c + pairs - 1) / pairs, of_dx = c < td ? (td - c + pairs - 1) / pairs : 0;
-            const long long t = of_dx * cd + (mine - of_dx) * cw + GLU_EPI_COST[2];
-            if (t > worst) worst = t;
-        }
-        if (td + tw >= pairs && worst <= least + least / 50) best = {1, -1};
-    }
-    return best;
-}
-// Workspace: dG and dU, then dx's parts.
-static uint64_t glu_half(unsigned n, unsigned m) { return (uint64_t(n) * m * 2 + 255) / 256 * 256; }
+// Pairs of SMs on the current device: one cluster each.
+static int glu_pairs() { return sm_count() < 2 ? 1 : sm_count() / 2; }
 
 static cudaError_t glu_check(unsigned n, unsigned k, unsigned m, unsigned type, unsigned act) {
     if ((type != EG_F16 && type != EG_BF16) || act > 1 || !k || !m || k % 8 || m % 8 || n > 0x7fffff00u ||
@@ -104,7 +52,7 @@ static cudaError_t glu_project(const void *x, int64_t xs, const void *wg, int64_
                                unsigned type, unsigned act, GluParams &p, cudaStream_t s) {
     GluMaps maps{};
     // The width whose slowest cluster is done first; the wider one where they tie.
-    const int pairs = sm_count() / 2, steps = ceil_div(p.k, 64);
+    const int pairs = glu_pairs(), steps = ceil_div(p.k, 64);
     int bn = 256;
     long long best = LLONG_MAX;
     for (int i = 2; i >= 0; --i) {
@@ -183,8 +131,9 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
         (a.dx && !glu_matrix_ok(a.dx, &dxs, a.k, a.n, 2)))
         return cudaErrorInvalidValue;
     if (!a.dx && !a.dw_gate && !a.dw_up) return cudaSuccess;
+    const int most = glu_most_splits(a.n, a.k, a.m);
     if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255) ||
-        a.workspace_bytes < eg2_glu_grad_workspace(a.n, a.k, a.m))
+        a.workspace_bytes < glu_grad_bytes(a.n, a.k, a.m, most))
         return cudaErrorInvalidValue;
     uint8_t *dg = static_cast<uint8_t *>(a.workspace), *du = dg + glu_half(a.n, a.m);
     GluParams p{};
@@ -201,8 +150,9 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
     p.out[0] = a.dx, p.out[1] = a.dw_gate, p.out[2] = a.dw_up;
     p.out_stride[0] = dxs, p.out_stride[1] = dgs, p.out_stride[2] = dus;
     p.dw_f32 = a.dw_type == EG_F32, p.dw_accumulate = a.accumulate != 0;
-    const int weights = (a.dw_gate != nullptr) + (a.dw_up != nullptr), pairs = sm_count() / 2;
-    const GluPlan plan = glu_plan(a.n, a.k, a.m, a.dx != nullptr, weights, pairs < GLU_PAIRS ? pairs : GLU_PAIRS);
+    const int weights = (a.dw_gate != nullptr) + (a.dw_up != nullptr);
+    const int pairs = glu_pairs() < GLU_PAIRS ? glu_pairs() : GLU_PAIRS;
+    const GluPlan plan = glu_plan(a.n, a.k, a.m, a.dx != nullptr, weights, pairs, most);
     const int w_tiles = weights * glu_tiles(a.m, a.k, 256);
     p.splits = plan.splits, p.parts = reinterpret_cast<float *>(dg + 2 * glu_half(a.n, a.m));
     p.dx_tiles = a.dx ? glu_tiles(a.n, a.k, 256) * plan.splits : 0;
@@ -228,13 +178,7 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
 extern "C" {
 int eg2_launch_glu(const EgGlu *p, void *s) { return rc(glu(*p, S(s))); }
 uint64_t eg2_glu_grad_workspace(unsigned n, unsigned k, unsigned m) {
-    if (!n || !k || !m) return 0;
-    int splits = 1;  // the most that dx, alone or beside one or both weights' gradients, may take
-    for (int w = 0; w <= 2; ++w) {
-        const int s = glu_plan(n, k, m, true, w, GLU_PAIRS).splits;
-        if (s > splits) splits = s;
-    }
-    return 2 * glu_half(n, m) + (splits > 1 ? uint64_t(splits) * n * k * 4 : 0);
+    return n && k && m ? glu_grad_bytes(n, k, m, glu_most_splits(n, k, m)) : 0;
 }
 int eg2_launch_glu_grad(const EgGluGrad *p, void *s) { return rc(glu_grad(*p, S(s))); }
 }
