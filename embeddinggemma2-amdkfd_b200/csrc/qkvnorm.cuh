@@ -292,7 +292,9 @@ __global__ void __launch_bounds__(256, 2) qkv_stream_kernel(const __grid_constan
                 }
 #pragma unroll
                 for (int h = 0; h < JOIN; ++h) {
-                    const float r = keep ? rsqrtf(ss[h] * inv_d + p.eps) : 0.0f;
+                    // A block's missing heads are rows of zeros: r = 0 there, for without
+                    // eps it would be infinite, and 0 * r would enter the weights' gradients.
+                    const float r = keep && h1 + h < live ? rsqrtf(ss[h] * inv_d + p.eps) : 0.0f;
                     const float m = GRAD ? -r * (r * r * (ux[h] * inv_d)) : 0.0f;
                     const float2 r2 = make_float2(r, r), m2 = make_float2(m, m);
 #pragma unroll

@@ -1,0 +1,46 @@
+"""The typed operators at the edges of what they accept, against their
+definitions in 64 bits.  The references and their bounds are those of
+test_gpu_typed_rows.py and test_gpu_glu.py."""
+import importlib
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import test_gpu_typed_rows as rows  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DEV, U = rows.DEV, rows.U
+F32, F16, BF16 = rows.F32, rows.F16, rows.BF16
+
+
+@pytest.fixture(scope="module")
+def ops(eg2):
+    return importlib.import_module("embeddinggemma2-amdkfd_b200.ops")
+
+
+# ---------------------------------------------------------------- qkv_norm_rope
+@pytest.mark.parametrize("n,hq,hkv,d", [(40, 1, 1, 128), (301, 3, 1, 64), (33, 5, 3, 96), (70, 3, 1, 512),
+                                        (50, 3, 1, 34)])
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (F16, F16)])
+def test_qkv_norm_rope_grad_without_eps(ops, monkeypatch, n, hq, hkv, d, dtype, wdtype):
+    """eps = 0 and head counts that do not fill the last block of heads: every row that is
+    there is nonzero, so both gradients are finite and within the bounds of any eps."""
+    monkeypatch.setattr(rows, "EPS", 0.0)
+    q, k, v, qw, kw, cos, sin, pos, g = rows.qkv_inputs(n, hq, hkv, d, dtype, wdtype, 5 * n + d)
+    gs = [rows.randn(t.shape, g, dtype) for t in (q, k, v)]
+    dx = [torch.full_like(t, 7.0) for t in gs]
+    dws = [torch.full((d,), 7.0, dtype=wdtype, device=DEV) for _ in range(2)]
+    ops.qkv_norm_rope_grad(*dx, *dws, *gs, q, k, v, qw, kw, cos, sin, pos, 0.0)
+    outs = [torch.full_like(t, 7.0) for t in gs]
+    ops.qkv_norm_rope(*outs, q, k, v, qw, kw, cos, sin, pos, 0.0)
+    rows.check_forward(outs, (q, k, v), (qw, kw, None), cos, sin, pos, dtype)
+    keep, c, s = rows.rope_rows(cos, sin, pos)
+    for kind, (x, w) in enumerate(((q, qw), (k, kw), (v, None))):
+        ref, mag, terms, tmag = rows.qkv_grad_ref(x, w, c if kind < 2 else None, s, gs[kind])
+        ref, mag = torch.where(keep, ref, 0.0), torch.where(keep, mag, 0.0)
+        rows.assert_within(dx[kind], ref, mag * 80 * U + rows.half_unit(ref, dtype), f"dx {kind}")
+        if kind < 2:
+            total, bound = (torch.where(keep, t, 0.0).sum((0, 1)) for t in (terms, tmag))
+            rows.assert_within(dws[kind], total,
+                               bound * (n * x.shape[1] + 24) * U + rows.half_unit(total, wdtype), f"dw {kind}")
