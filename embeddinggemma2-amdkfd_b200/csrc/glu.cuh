@@ -136,14 +136,16 @@ template <int ACT>
 __device__ __forceinline__ float glu_act(float g) {
     return ACT == ACT_SILU ? g * logistic(g) : g * logistic(g * fmaf(GELU_B * g, g, GELU_A));
 }
-// act(g) and act'(g) = s (1 + g z' (1 - s)).
+// act(g) and act'(g) = s (1 + g z' (1 - s)).  gelu's slope is 0 or 1, and s too, to
+// the last bit of fp32 beyond |g| = 32; held there (NaN stays NaN), since g z'
+// overflows from |g| = 1.2e13 and 0 * inf would be NaN.
 template <int ACT>
 __device__ __forceinline__ float glu_act_grad(float g, float *act) {
-    const float g2 = g * g;
-    const float s = logistic(ACT == ACT_SILU ? g : g * fmaf(GELU_B, g2, GELU_A));
-    const float dz = ACT == ACT_SILU ? 1.0f : fmaf(3.0f * GELU_B, g2, GELU_A);
+    const float b = ACT == ACT_SILU || !(fabsf(g) > 32.0f) ? g : copysignf(32.0f, g), b2 = b * b;
+    const float s = logistic(ACT == ACT_SILU ? b : b * fmaf(GELU_B, b2, GELU_A));
+    const float dz = ACT == ACT_SILU ? 1.0f : fmaf(3.0f * GELU_B, b2, GELU_A);
     *act = g * s;
-    return s * fmaf(g * dz, 1.0f - s, 1.0f);
+    return s * fmaf(b * dz, 1.0f - s, 1.0f);
 }
 // ---------------------------------------------------------------- tiles
 // kind 0: the projections' tile or dx's; kinds 1 and 2: dWg's and dWu's.

@@ -6,6 +6,7 @@ import importlib
 import pytest
 
 torch = pytest.importorskip("torch")
+import test_gpu_glu as gated  # noqa: E402
 import test_gpu_typed_rows as rows  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +45,34 @@ def test_qkv_norm_rope_grad_without_eps(ops, monkeypatch, n, hq, hkv, d, dtype, 
             total, bound = (torch.where(keep, t, 0.0).sum((0, 1)) for t in (terms, tmag))
             rows.assert_within(dws[kind], total,
                                bound * (n * x.shape[1] + 24) * U + rows.half_unit(total, wdtype), f"dw {kind}")
+
+
+# ---------------------------------------------------------------- glu
+@pytest.mark.parametrize("n", [2, 14, 300])
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
+def test_glu_grad_of_large_gates(ops, n, act):
+    """Gates up to 1e17, past where their cubes overflow fp32: the slope is 1 on one side and
+    0 on the other.  Each projection is one product, so G and U are exact and only the
+    roundings behind them are left of the bounds."""
+    k, m, g = 64, 136, gated.gen(n)
+    x = torch.zeros((n, k), dtype=BF16, device=DEV)
+    big = torch.tensor([300.0, -300.0, 1e6, -1e6, 1e12, -1e12, 1.3e13, -1.3e13, 1e14, -1e14, 3e15, -3e15, 1e17, -1e17],
+                       device=DEV)
+    x[:, 0] = big[torch.arange(n, device=DEV) % 14 if n > 2 else slice(8, 10)].to(BF16)
+    x[:, 1] = gated.randn((n,), g, BF16)
+    wg, wu = torch.zeros((m, k), dtype=BF16, device=DEV), torch.zeros((m, k), dtype=BF16, device=DEV)
+    wg[:, 0] = 1.0
+    wu[:, 1] = gated.randn((m,), g, BF16)
+    dout = gated.randn((n, m), g, BF16)
+    got = [torch.full_like(t, 7.0) for t in (x, wg, wu)]
+    ops.glu_grad(*got, dout, x, wg, wu, act)
+    ref = gated.Ref(x, wg, wu, act, BF16)
+    ref.eg, ref.eu = torch.zeros_like(ref.eg), torch.zeros_like(ref.eu)
+    for name, a, (r, e) in zip(("dx", "dw_gate", "dw_up"), got, ref.backward(dout, BF16)):
+        gated.assert_within(a, r, e, name)
+    # A gate that is not a number stays one, in its row and column only.
+    wg[5, 0] = float("nan")
+    dw = torch.empty_like(wg)
+    ops.glu_grad(None, dw, None, dout, x, wg, wu, act)
+    assert dw[5, :2].isnan().all() and torch.equal(dw[:5], got[1][:5]) and torch.equal(dw[6:], got[1][6:])
+    assert ops.read_error() == 0
