@@ -87,18 +87,20 @@ __device__ __forceinline__ bool bar_try_wait(uint64_t *bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Every wait on a barrier is bounded: after ~2 s (or, when abort is given,
-// once another thread of the CTA gave up) it returns false and records
+// Every wait on a barrier is bounded: after ~2 s, or the limit given (or, when abort
+// is given, once another thread of the CTA gave up) it returns false and records
 // ERR_WAIT_TIMEOUT, so a lost arrival can never hang the GPU.  Waits used to
 // drain this CTA's own in-flight copies / MMAs before exit pass abort = nullptr.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *abort) {
+constexpr uint64_t WAIT_NS = 2000000000ull;
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *abort,
+                                         uint64_t limit_ns = WAIT_NS) {
     if (bar_try_wait(bar, parity)) return true;
     const uint64_t start = globaltimer_ns();
     for (uint32_t i = 1;; ++i) {
         if (bar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 0) {
             if (abort && *abort) return false;
-            if (globaltimer_ns() - start > 2000000000ull) {
+            if (globaltimer_ns() - start > limit_ns) {
                 if (abort) *abort = 1;
                 atomicExch(&g_error, ERR_WAIT_TIMEOUT);
                 return false;

@@ -339,7 +339,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<MODE, BN>::TH
                         dh[c] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.dout) + r * p.dout_stride + col);
                 }
             }
-            if (!__all_sync(0xffffffffu, wait_bar(&accfull[buf], (ti >> 1) & 1, abort))) break;
+            // The one wait for a whole tile's products: 2 us a step on top of the usual
+            // limit, about six times what a step takes, since K may be 2^25 steps long.
+            const uint64_t limit = WAIT_NS + uint64_t(t.steps) * 2000;
+            if (!__all_sync(0xffffffffu, wait_bar(&accfull[buf], (ti >> 1) & 1, abort, limit))) break;
             tc_fence_after();
             // The accumulator is free for the tile after next once both CTAs' warps have read it.
             auto release = [&] {

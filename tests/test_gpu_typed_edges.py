@@ -76,3 +76,25 @@ def test_glu_grad_of_large_gates(ops, n, act):
     ops.glu_grad(None, dw, None, dout, x, wg, wu, act)
     assert dw[5, :2].isnan().all() and torch.equal(dw[:5], got[1][:5]) and torch.equal(dw[6:], got[1][6:])
     assert ops.read_error() == 0
+
+
+def test_glu_grad_of_very_many_rows(ops):
+    """600 million rows: a weight gradient's tile is 9.4 million K steps, near three seconds
+    of products.  All rows but a few are zero, the last one not, so the sums are theirs."""
+    n, k, m = 600_000_000, 8, 8
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip("needs 48 GB")
+    g = gated.gen(3)
+    live = torch.tensor([0, 5, n // 2, n - 65, n - 1], device=DEV)
+    x = torch.zeros((n, k), dtype=BF16, device=DEV)
+    dout = torch.ones((n, m), dtype=BF16, device=DEV)
+    x[live], dout[live] = gated.randn((5, k), g, BF16), gated.randn((5, m), g, BF16)
+    wg, wu = gated.randn((m, k), g, BF16), gated.randn((m, k), g, BF16)
+    dw = [torch.full((m, k), 7.0, device=DEV) for _ in range(2)]
+    ops.glu_grad(None, *dw, dout, x, wg, wu)
+    ref = gated.Ref(x[live], wg, wu, "gelu_tanh", BF16).backward(dout[live], F32)[1:]
+    for name, a, (r, e) in zip(("dw_gate", "dw_up"), dw, ref):
+        gated.assert_within(a, r, e, name)
+    assert ops.read_error() == 0
+    del x, dout
+    torch.cuda.empty_cache()
