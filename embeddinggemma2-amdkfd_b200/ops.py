@@ -399,7 +399,8 @@ def glu_grad(dx, dw_gate, dw_up, dout, x, w_gate, w_up, act="gelu_tanh", accumul
     projections are computed again."""
     n, k, m, dev, dtype, code, strides = _glu_args(x, w_gate, w_up, act)
     dout_stride = _check(dout, "dout", (n, m), dev, dtype)[0]
-    dw_type = dw_gate.dtype if dw_gate is not None else dw_up.dtype if dw_up is not None else dtype
+    # Where neither is wanted there is nothing to add to, and accumulate says nothing.
+    dw_type = dw_gate.dtype if dw_gate is not None else dw_up.dtype if dw_up is not None else torch.float32
     if dw_type not in (torch.float32, dtype) or (accumulate and dw_type != torch.float32):
         raise ValueError(f"weight gradients are {dw_type}: expected float32" + ("" if accumulate else f" or {dtype}"))
     dx_stride = 0 if dx is None else _check(dx, "dx", (n, k), dev, dtype)[0]

@@ -98,3 +98,15 @@ def test_glu_grad_of_very_many_rows(ops):
     assert ops.read_error() == 0
     del x, dout
     torch.cuda.empty_cache()
+
+
+def test_glu_grad_accumulates_with_frozen_weights(ops):
+    """dx alone with accumulate: there is no weight gradient to be of a wrong type, and dx is written."""
+    x, wg, wu, dout = gated.inputs(70, 64, 72, F16, 4)
+    a, b = torch.full_like(x, 7.0), torch.full_like(x, -7.0)
+    ops.glu_grad(a, None, None, dout, x, wg, wu, accumulate=True)
+    ops.glu_grad(b, None, None, dout, x, wg, wu)
+    assert torch.equal(a, b)
+    r, e = gated.Ref(x, wg, wu, "gelu_tanh", F16).backward(dout, F32)[0]
+    gated.assert_within(a, r, e)
+    ops.glu_grad(None, None, None, dout, x, wg, wu, accumulate=True)  # nothing wanted
