@@ -273,7 +273,7 @@ static cudaError_t qkv_common(QkvNormParams *p, bool *wide, unsigned n, const un
         q.x_tok = xs[i][0], q.x_head = xs[i][1], q.out_tok = outs[i][0], q.out_head = outs[i][1];
         if (q.w && !aligned16(q.w)) *wide = false;
         if (i < 2) {
-            if (!rc || !rs) return cudaErrorInvalidValue;
+            if (positions && (!rc || !rs)) return cudaErrorInvalidValue;  // no rows: never read
             if (!aligned16(rc) || !aligned16(rs)) *wide = false;
         }
     }

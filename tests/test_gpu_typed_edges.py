@@ -47,6 +47,22 @@ def test_qkv_norm_rope_grad_without_eps(ops, monkeypatch, n, hq, hkv, d, dtype, 
                                bound * (n * x.shape[1] + 24) * U + rows.half_unit(total, wdtype), f"dw {kind}")
 
 
+@pytest.mark.parametrize("n,d", [(5, 64), (9001, 512), (40, 34)])
+def test_qkv_norm_rope_with_empty_tables(ops, n, d):
+    """Tables without rows: every position is padding, so all is zero and nothing is read."""
+    x = torch.full((n, 4, d), float("nan"), device=DEV)
+    none = torch.empty((0, d // 2), device=DEV)
+    pos = torch.arange(n, device=DEV, dtype=torch.int32) - 2
+    w = torch.ones(d, device=DEV)
+    parts = lambda t: (t[:, :2], t[:, 2:3], t[:, 3:])
+    out, dx = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    dws = [torch.full((d,), 7.0, device=DEV) for _ in range(2)]
+    ops.qkv_norm_rope(*parts(out), *parts(x), w, w, none, none, pos)
+    ops.qkv_norm_rope_grad(*parts(dx), *dws, *parts(x), *parts(x), w, w, none, none, pos)
+    for t in (out, dx, *dws):
+        assert (t == 0).all()
+
+
 # ---------------------------------------------------------------- glu
 @pytest.mark.parametrize("n", [2, 14, 300])
 @pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
