@@ -126,10 +126,12 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
         }
         return cudaSuccess;
     }
+    const bool one_row = a.dout_stride == 0;  // a broadcast gradient; dout is read by plain loads, not through a map
     if (!glu_matrix_ok(a.x, &xs, a.k, a.n, 2) || !glu_matrix_ok(a.w_gate, &gs, a.k, a.m, 2) ||
-        !glu_matrix_ok(a.w_up, &us, a.k, a.m, 2) || !glu_matrix_ok(a.dout, &os, a.m, a.n, 2) ||
+        !glu_matrix_ok(a.w_up, &us, a.k, a.m, 2) || !glu_matrix_ok(a.dout, &os, a.m, one_row ? 1 : a.n, 2) ||
         (a.dx && !glu_matrix_ok(a.dx, &dxs, a.k, a.n, 2)))
         return cudaErrorInvalidValue;
+    if (one_row) os = 0;
     if (!a.dx && !a.dw_gate && !a.dw_up) return cudaSuccess;
     const int most = glu_most_splits(a.n, a.k, a.m);
     if (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255) ||

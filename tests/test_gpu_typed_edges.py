@@ -126,3 +126,17 @@ def test_glu_grad_accumulates_with_frozen_weights(ops):
     r, e = gated.Ref(x, wg, wu, "gelu_tanh", F16).backward(dout, F32)[0]
     gated.assert_within(a, r, e)
     ops.glu_grad(None, None, None, dout, x, wg, wu, accumulate=True)  # nothing wanted
+
+
+@pytest.mark.parametrize("n", [1, 2, 70, 700])
+def test_glu_grad_of_a_broadcast_gradient(ops, n):
+    """One row of dout for all tokens (row stride 0): the bits of the same rows written out."""
+    x, wg, wu, dout = gated.inputs(n, 64, 136, BF16, n)
+    row = dout[:1].expand(n, 136)
+    got, want = ([torch.full_like(t, 7.0) for t in (x, wg, wu)] for _ in range(2))
+    ops.glu_grad(*got, row, x, wg, wu)
+    ops.glu_grad(*want, row.contiguous(), x, wg, wu)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for a, (r, e) in zip(got, gated.Ref(x, wg, wu, "gelu_tanh", BF16).backward(row, BF16)):
+        gated.assert_within(a, r, e)
