@@ -87,9 +87,10 @@ struct EmbedGradLayout {
 };
 static EmbedGradLayout embed_grad_layout(unsigned n, unsigned d) {
     EmbedGradLayout L{};
-    // About 8 warps on each of 148 SMs, a warp for 256 columns of a chunk; 8 items at least.
-    const long long warps = 8 * 148, share = ceil_div((long long)n * ceil_div(d, 256), warps);
-    L.chunk = int((share < 8 ? 8 : share) + 7) / 8 * 8;
+    // About 8 warps on each of 148 SMs, a warp for 256 columns of a chunk; 8 items at
+    // least, and no more than there are (a share passes 2^31 for many wide rows).
+    const long long warps = 8 * 148, share = ((long long)n * ceil_div(d, 256) + warps - 1) / warps;
+    L.chunk = int(((share < 8 ? 8 : share > n ? n : share) + 7) / 8 * 8);
     L.chunks = ceil_div(n, L.chunk);
     L.subtiles = ceil_div(n, (long long)EmbedSort::SUB * EmbedSort::MAX_TILES);
     if (L.subtiles < 1) L.subtiles = 1;
