@@ -279,6 +279,8 @@ static cudaError_t qkv_common(QkvNormParams *p, bool *wide, unsigned n, const un
         }
     }
     if (n && !pos) return cudaErrorInvalidValue;
+    // At least 8 rows a CTA in both directions: fewer than 2^31 CTAs, or items of them.
+    if (((long long)n * (p->part[0].heads + p->part[1].heads + p->part[2].heads)) >> 33) return cudaErrorInvalidValue;
     p->rope_cos = rc, p->rope_sin = rs, p->pos = pos;
     p->n = int(n), p->d = int(d), p->positions = int(positions), p->weight_f32 = weight_type == EG_F32, p->eps = eps;
     return cudaSuccess;
@@ -331,7 +333,6 @@ static cudaError_t qkv_norm_rope(const EgQkvNormRope &a, cudaStream_t s) {
         return e;
     const long long rows = (long long)p.n * (p.part[0].heads + p.part[1].heads + p.part[2].heads);
     if (!rows) return cudaSuccess;
-    if (rows >> 33) return cudaErrorInvalidValue;  // at least 8 rows a CTA: fewer than 2^31 CTAs
     return by_type(a.type, [&](auto t) {
         using T = typename decltype(t)::type;
         return qkv_shape<T>(p.d / 2, wide, [&](auto v, auto g, auto nv) {

@@ -147,8 +147,8 @@ typedef struct {
  * (token, head).  A head count of 0 leaves that tensor out; a null weight is 1.
  * A position outside [0, positions) is padding: zeros, and x is not read (with
  * positions = 0 all are, and the tables may be null).  d even, at most 512; n at
- * most 2^30; weight_type is EG_F32 or type.  Strides are
- * not negative; out may be x itself. */
+ * most 2^30, rows of all heads together fewer than 2^33; weight_type is EG_F32 or
+ * type.  Strides are not negative; out may be x itself. */
 typedef struct {
     void *out[3]; const void *x[3]; const void *weight[2]; const float *rope_cos, *rope_sin; const int *pos;
     int64_t out_stride[3][2], x_stride[3][2];
