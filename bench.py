@@ -198,10 +198,20 @@ def wave_rows(n, seed):
     return np.random.default_rng(seed).standard_normal((n, 512)).astype(np.float32)
 
 
+def unavailable(path):
+    """Why a build of the reference cannot run, in one line, or None where it is there."""
+    if os.path.exists(path):
+        return None
+    return f"{os.path.relpath(path, ROOT)} is not built: it is made from the reference's sources, which are not here"
+
+
 def cpu_baseline_run(model_path, lengths, steps, warmup, seed, rows=False):
     """The reference's own CPU graph (oracle/_ref) on the same waves (with
-    rows: the same offsets, the graph started from input rows, ids NULL)."""
+    rows: the same offsets, the graph started from input rows, ids NULL).
+    Where that is not built: {"unavailable": why}."""
     import oracle
+    if unavailable(oracle.REF_SO):
+        return {"unavailable": unavailable(oracle.REF_SO)}
     syn = importlib.import_module("embeddinggemma2-amdkfd_b200.synthetic")
     ids, off = syn.wave(lengths, seed=seed)
     ref = oracle.RefGraph(model_path, 0)
@@ -436,10 +446,14 @@ def reference_arm(args, rank, world):
         return
     if args.config == 5:
         return reference_arm_attention(args)
-    if args.config == 3:
-        return reference_arm_mixed(args)
     if args.config == 4:
         return reference_arm_gemm(args)
+    import oracle
+    if unavailable(oracle.REF_SO):
+        print(json.dumps({"impl": "reference", "unavailable": unavailable(oracle.REF_SO)}), flush=True)
+        return
+    if args.config == 3:
+        return reference_arm_mixed(args)
     syn = importlib.import_module("embeddinggemma2-amdkfd_b200.synthetic")
     desc, lengths = CONFIGS[args.config]
     model = syn.model_path(1234, "baseline")
@@ -792,6 +806,9 @@ def http_run(args, reference=False):
     n_srv = 1 if reference or cuda else args.gpus
     model_path = syn.model_path(1234, "baseline", tokenizer=True)
     binary = SERVER_CPU_BIN if reference else SERVER_CUDA_BIN if cuda else SERVER_BIN
+    if reference and unavailable(binary):
+        print(json.dumps({"impl": "reference", "unavailable": unavailable(binary)}), flush=True)
+        return
     if not os.path.exists(binary):
         raise SystemExit(f"{binary} missing: make -C oracle server")
     backend = "cpu" if reference else "cuda" if cuda else "kfd"
