@@ -7,6 +7,7 @@
 //
 //   dG = dout U act'(G), dU = dout act(G)              (GLU_DGRAD: rounded once to the operands' type,
 //                                                       since the next products take them as operands)
+//                                                       (in fp16 infinite above 65504)
 //   dx = dG Wg + dU Wu, dWg = dG^T x, dWu = dU^T x     (GLU_PRODUCTS)
 //
 // act is gelu_tanh(g) = g s(2 c (g + 0.044715 g^3)), c = sqrt(2/pi), or silu(g) =

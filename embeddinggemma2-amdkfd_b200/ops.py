@@ -396,7 +396,8 @@ def glu_grad(dx, dw_gate, dw_up, dout, x, w_gate, w_up, act="gelu_tanh", accumul
 
     The weights' gradients are of x's type or float32; with accumulate they are
     float32 and added to.  Nothing is kept from the forward pass: the
-    projections are computed again."""
+    projections are computed again, and their gradients are rounded to x's type
+    (in float16 one above 65504 is infinite, and so are the rows it enters)."""
     n, k, m, dev, dtype, code, strides = _glu_args(x, w_gate, w_up, act)
     dout_stride = _check(dout, "dout", (n, m), dev, dtype)[0]
     # Where neither is wanted there is nothing to add to, and accumulate says nothing.

@@ -179,8 +179,10 @@ typedef struct {
  * computed again, so nothing is kept from the forward pass.  dx [n][k] (type),
  * dw_gate and dw_up [m][k] (dw_type: type or EG_F32; with accumulate, EG_F32
  * only, added to what they hold); any of the three may be null.  The
- * projections' gradients are rounded once to type between the two steps.  dout's
- * row stride may be 0: one row for all tokens.
+ * projections' gradients are rounded once to type between the two steps; one
+ * that leaves EG_F16's range (above 65504) is infinite there, and its token's row
+ * of dx and its row of dw are then not finite, so scale an fp16 loss as usual.
+ * dout's row stride may be 0: one row for all tokens.
  * workspace: eg2_glu_grad_workspace(n, k, m) bytes. */
 typedef struct {
     void *dx, *dw_gate, *dw_up; const void *dout, *x, *w_gate, *w_up; void *workspace; uint64_t workspace_bytes;

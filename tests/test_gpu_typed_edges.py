@@ -140,3 +140,28 @@ def test_glu_grad_of_a_broadcast_gradient(ops, n):
         assert torch.equal(a, b)
     for a, (r, e) in zip(got, gated.Ref(x, wg, wu, "gelu_tanh", BF16).backward(row, BF16)):
         gated.assert_within(a, r, e)
+
+
+@pytest.mark.parametrize("dw", [F16, F32])
+def test_glu_grad_past_the_range_of_fp16(ops, dw):
+    """A projection's gradient above 65504 shows: its token's row of dx and its row of dw_gate
+    are not finite, never a wrong finite number, and all other rows keep their bits."""
+    n, k, m, t, c = 70, 64, 136, 33, 77
+    x, wg, wu, dout = gated.inputs(n, k, m, F16, 6)
+    x[t], wg[c], wu[c] = 1.0, 0.25, 0.25                       # G = U = 16 there, act'(G) = 1
+    got, want = ([torch.full_like(x, 7.0), *(torch.full((m, k), 7.0, dtype=dw, device=DEV) for _ in range(2))]
+                 for _ in range(2))
+    dout[t, c] = 0.0
+    ops.glu_grad(*want, dout, x, wg, wu)
+    dout[t, c] = 3900.0                                        # dG = 62400, dU = 62400: the last that fit
+    ops.glu_grad(*got, dout, x, wg, wu)
+    assert all(a.isfinite().all() for a in got)
+    for a, (r, e) in zip(got, gated.Ref(x, wg, wu, "gelu_tanh", F16).backward(dout, dw)):
+        gated.assert_within(a, r, e)
+    dout[t, c] = 4200.0                                        # 67200
+    ops.glu_grad(*got, dout, x, wg, wu)
+    dx, dwg, dwu = got
+    assert not (dx[t].isfinite().any() or dwg[c].isfinite().any() or dwu[c].isfinite().any())
+    other, rest = torch.arange(n, device=DEV) != t, torch.arange(m, device=DEV) != c
+    assert torch.equal(dx[other], want[0][other])
+    assert torch.equal(dwg[rest], want[1][rest]) and torch.equal(dwu[rest], want[2][rest])
