@@ -6,8 +6,10 @@
 
 namespace eg2 {
 
-// Up to this many rows run on the CUDA cores: 4 rows x 2048 x 8192 take no longer
-// there than on the tensor cores (about 19 us), 8 took 34 against 20.
+// Up to this many rows run on the CUDA cores.  Weights from memory, us on the CUDA
+// cores for 1, 2, 3, 4, 5 and 8 rows against the tensor cores' (the same for all):
+// 512 x 2048 2.5, 3.4, 4.2, 3.4, 4.1, 5.2 against 7.3; 2048 x 8192 15.1, 19.1, 23.4,
+// 17.6, 31.4, 38.7 against 21.2.
 constexpr unsigned GLU_FEW_ROWS = 4;
 
 // [rows][width] of a 16-bit type, boxes of 64 elements x box_rows, 128-byte swizzle.
@@ -65,7 +67,9 @@ static cudaError_t glu_project(const void *x, int64_t xs, const void *wg, int64_
         !glu_tmap(&maps.wu, type, wu, wus, unsigned(p.k), unsigned(p.m), wrows))
         return cudaErrorInvalidValue;
     p.tiles = glu_tiles(unsigned(p.n), unsigned(p.m), bn / 2);
-    p.group = 16;  // 16411 x 2048 x 8192: 832 us, 852 with 8 (the weights are read half as often), 829 with 32
+    // 16411 x 2048 x 8192: 738 us, 751 with 8 (the weights are read half as often), 732
+    // with 32; 8192 x 4096 x 4096 353, 360 and 375; 4096 x 2048 x 16384 362, 371 and 365.
+    p.group = 16;
     const int clusters = p.tiles < pairs ? p.tiles : pairs;
     return glu_dispatch(type, act, [&](auto t, auto a) {
         using T = typename decltype(t)::type;
@@ -163,7 +167,10 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
     const int w_clusters = pairs - (plan.dxc < 0 ? 0 : plan.dxc);
     const int clusters = plan.dxc < 0 ? pairs : p.dx_clusters + (w_tiles < w_clusters ? w_tiles : w_clusters);
     // Whole rows of tiles where those are few: 8203 x 2048 x 8192 (8 tiles a row) takes
-    // 1353 us with 1, 1372 with 8, 1405 with 16.
+    // 1206 us with 1, 1235 with 8, 1250 with 16, 4096 x 2304 x 4096 (9) 344 and 363 with 1
+    // and 8.  Bands of 8 where they are many: 8192 x 4096 x 8192 (16 tiles) 2.71 and 2.49
+    // ms, 2048 x 8192 x 8192 (32) 1.40 and 1.25 ms.  In between neither is ahead by more
+    // than runs differ (4096 rows, m = 4096: 10 tiles 401 and 432 us, 16 tiles 615 and 614).
     p.group = ceil_div(a.k, 256) <= 9 ? 1 : 8;
     return glu_dispatch(a.type, 0, [&](auto t, auto) {
         using T = typename decltype(t)::type;

@@ -134,10 +134,13 @@ static cudaError_t embed_rows_grad(const EgEmbedRowsGrad &a, cudaStream_t s) {
     q.hist = reinterpret_cast<unsigned *>(ws + L.hist);
     q.n = int(a.n), q.vocab = int(a.vocab), q.tiles = L.tiles, q.subtiles = L.subtiles, q.bits = bits;
     // The table's untouched rows are cleared beside the other work: beside the sort
-    // about what can be written in the time that it takes anyway (64 MB a scatter: 93
-    // us at 100003 tokens, 95 with 32 or 134 MB, 96 also beside the histograms), the
-    // rest beside the sums.  A larger vocabulary than there are flags for is
-    // cleared whole before the sums.
+    // about what can be written in the time that it takes anyway, the rest beside the
+    // sums.  262144 x 512 bf16, uniform ids: 96 MB beside the small sort 49 us at 1999
+    // tokens and 52 at 4096, with 48 MB 50 and 58, with none 58 and 65; 64 MB a scatter
+    // 59 us at 5000 tokens and 71 at 40000, with none 65 and 75, at 100003 95 either
+    // way, at 300000 167 against 157, where the sums have the time.  (Natural ids at
+    // 100003: 93 us, 95 with 32 or 134 MB, 96 also beside the histograms.)  A larger
+    // vocabulary than there are flags for is cleared whole before the sums.
     const bool flags_fit = a.vocab <= EmbedSort::MAX_TOUCHED;
     uint8_t *touched = a.accumulate || !flags_fit ? nullptr : ws + L.touched;
     const long long block_bytes = 8ll * a.d * sw;

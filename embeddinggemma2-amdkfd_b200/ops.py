@@ -134,8 +134,10 @@ def pool_l2(out, y, offsets, batch, width):
 
 
 # ---- typed operators and their gradients (fp32, fp16, bf16) ----
-# These check their tensors (ValueError before anything is enqueued) and run on
-# the current stream of their tensors' device, whichever device is current.  A
+# These check their tensors' shapes, types, devices and rows (ValueError) and leave
+# alignment, overlapping rows and limits to the C entry point (RuntimeError); both
+# before anything is enqueued.  They run on the current stream of their tensors'
+# device, whichever device is current, and record nothing for autograd.  A
 # call of a small operator is mostly host time, so a check that passes is a few
 # comparisons, and the parameters are packed straight into the C struct's bytes.
 class _Typed:
@@ -162,6 +164,9 @@ class _Typed:
         else:
             with torch.cuda.device(index):
                 rc = self.fn(params, torch._C._cuda_getCurrentRawStream(index))
+        if rc == 1:  # cudaErrorInvalidValue, before anything is enqueued
+            raise RuntimeError(f"{self.name} refused its arguments (CUDA error 1): rows that overlap or are not "
+                               "aligned as it needs, or sizes past its limits")
         if rc:
             raise RuntimeError(f"{self.name} failed with CUDA error {rc}")
 
@@ -254,7 +259,8 @@ def embed_rows_grad(dtable, dout, ids, scale=1.0, accumulate=False, workspace=No
     """dtable[v] = scale * sum of dout[t] over ids[t] = v, or added to dtable (accumulate).
 
     dtable [vocab][d] and dout [n][d] are float32, float16 or bfloat16 (each its
-    own), ids int32 [n]; the sums are in fp32, in token order."""
+    own), ids int32 [n]; the sums are in fp32 and the same inputs give the same
+    bits.  dout may be broadcast over tokens (row stride 0)."""
     (vocab, d), dev, stride = _lead(dtable, "dtable", 2)
     n, dout_stride = _rows(dout, "dout", d, dev)
     _check(ids, "ids", (n,), dev, torch.int32)
@@ -325,7 +331,8 @@ def qkv_norm_rope(q_out, k_out, v_out, q, k, v, q_weight, k_weight, rope_cos, ro
     row pos[t] of rope_cos, rope_sin [positions][d / 2]; v gets the norm alone.
 
     Any of the three may be None with its output; a weight None is 1.  A position
-    outside the tables is padding (zeros).  An output may be its input."""
+    outside the tables is padding (zeros), so they are given for values alone
+    too.  An output may be its input."""
     sizes, dev, dtype = _qkv_args((q, k, v), q_weight, k_weight, rope_cos, rope_sin, pos)
     x, xs = _qkv_tensors(("q", "k", "v"), (q, k, v), sizes, dev, dtype)
     out, outs = _qkv_tensors(("q_out", "k_out", "v_out"), (q_out, k_out, v_out), sizes, dev, dtype)
@@ -394,6 +401,7 @@ def glu_grad_workspace(n, k, m) -> int:
 def glu_grad(dx, dw_gate, dw_up, dout, x, w_gate, w_up, act="gelu_tanh", accumulate=False, workspace=None):
     """The gradient of glu from dout [n][m] (None among dx, dw_gate, dw_up: not wanted).
 
+    dout may be broadcast over tokens (row stride 0).
     The weights' gradients are of x's type or float32; with accumulate they are
     float32 and added to.  Nothing is kept from the forward pass: the
     projections are computed again, and their gradients are rounded to x's type

@@ -130,8 +130,8 @@ typedef struct {
     void *out; const void *table; const int *ids; int64_t out_stride, table_stride;
     unsigned n, vocab, d, out_type, table_type; float scale;
 } EgEmbedRows;
-/* dtable[v] = scale * sum of dout[t] over ids[t] = v (in an order that n and d fix),
- * zero for an id that does not occur; with accumulate, added to what dtable
+/* dtable[v] = scale * sum of dout[t] over ids[t] = v (associated in a way that n, d
+ * and all of ids fix, so other ids in the batch can change its last bits), zero for an id that does not occur; with accumulate, added to what dtable
  * holds (rows that do not occur are then not touched).  Padding's rows of dout
  * are not read.  n is at most 2^30.  workspace:
  * eg2_embed_rows_grad_workspace(n, d) bytes. */

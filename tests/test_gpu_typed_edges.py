@@ -63,6 +63,22 @@ def test_qkv_norm_rope_with_empty_tables(ops, n, d):
         assert (t == 0).all()
 
 
+@pytest.mark.parametrize("shape", [(1, 1), (1, 3), (150, 1)])
+def test_qkv_norm_rope_grad_of_a_broadcast_gradient(ops, shape):
+    """dout with token stride 0, head stride 0 or both: the bits of the same rows written out."""
+    n, hq, hkv, d = 150, 3, 1, 64
+    q, k, v, qw, kw, cos, sin, pos, g = rows.qkv_inputs(n, hq, hkv, d, BF16, F32, 12)
+    gq = rows.randn((*shape, d), g, BF16).expand(n, hq, d)
+    gk, gv = (rows.randn((1, hkv, d), g, BF16).expand(n, hkv, d) for _ in range(2))
+    got, want = [], []
+    for out, grads in ((got, (gq, gk, gv)), (want, tuple(t.contiguous() for t in (gq, gk, gv)))):
+        out += [torch.full_like(t, 7.0, memory_format=torch.contiguous_format) for t in (q, k, v)]
+        out += [torch.full((d,), 7.0, device=DEV) for _ in range(2)]
+        ops.qkv_norm_rope_grad(*out, *grads, q, k, v, qw, kw, cos, sin, pos, 1e-6)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 # ---------------------------------------------------------------- glu
 @pytest.mark.parametrize("n", [2, 14, 300])
 @pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
