@@ -292,6 +292,8 @@ __global__ void __launch_bounds__(256, 2) qkv_stream_kernel(const __grid_constan
                 }
 #pragma unroll
                 for (int h = 0; h < JOIN; ++h) {
+                    // rsqrtf (two units of fp32) and 1 / d rounded once: below every 16-bit
+                    // type's rounding; an fp32 gradient is 1.5e-7 off, a plain form's 1.4e-7.
                     // A block's missing heads are rows of zeros: r = 0 there, for without
                     // eps it would be infinite, and 0 * r would enter the weights' gradients.
                     const float r = keep && h1 + h < live ? rsqrtf(ss[h] * inv_d + p.eps) : 0.0f;
