@@ -238,6 +238,12 @@ def _workspace(workspace, need, device):
     return ptr, size, workspace
 
 
+def _apart(a, b, names):
+    """Two gradients written by one call are two tensors: one given twice would lose a part of each."""
+    if a is not None and b is not None and a.data_ptr() == b.data_ptr() and a.numel():
+        raise ValueError(f"{names} are the same memory: each needs its own")
+
+
 def embed_rows(out, table, ids, scale=1.0):
     """out[t] = scale * table[ids[t]]; an id outside the table is padding (zeros).
 
@@ -361,6 +367,7 @@ def qkv_norm_rope_grad(dq, dk, dv, dq_weight, dk_weight, dq_out, dk_out, dv_out,
                 raise ValueError(f"{name} is wanted of a weight that is None")
             _check(w, name, (d,), dev, given.dtype)
             need = qkv_norm_rope_grad_workspace(n, hq, max(hk, hv), d)
+    _apart(dq_weight, dk_weight, "dq_weight and dk_weight")
     ws = _workspace(workspace, need, dev) if need else (0, 0, None)
     _qkv_norm_rope_grad(dev, *dx, _ptr(dq_weight), _ptr(dk_weight), *g, *x, _ptr(q_weight), _ptr(k_weight),
                         rope_cos.data_ptr(), rope_sin.data_ptr(), pos.data_ptr(), ws[0], ws[1], *dxs, *gs, *xs,
@@ -415,6 +422,7 @@ def glu_grad(dx, dw_gate, dw_up, dout, x, w_gate, w_up, act="gelu_tanh", accumul
     dx_stride = 0 if dx is None else _check(dx, "dx", (n, k), dev, dtype)[0]
     dg_stride = 0 if dw_gate is None else _check(dw_gate, "dw_gate", (m, k), dev, dw_type)[0]
     du_stride = 0 if dw_up is None else _check(dw_up, "dw_up", (m, k), dev, dw_type)[0]
+    _apart(dw_gate, dw_up, "dw_gate and dw_up")
     ws = _workspace(workspace, glu_grad_workspace(n, k, m), dev)
     _glu_grad(dev, _ptr(dx), _ptr(dw_gate), _ptr(dw_up), dout.data_ptr(), x.data_ptr(), w_gate.data_ptr(),
               w_up.data_ptr(), ws[0], ws[1], dx_stride, dg_stride, du_stride, dout_stride, *strides, n, k, m, code,

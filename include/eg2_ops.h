@@ -120,7 +120,8 @@ typedef struct { float *out; const float *y; const unsigned *offsets; unsigned b
  * numbers EG_F32, EG_F16, EG_BF16; strides count elements; the elements of a
  * row are contiguous.  Sums and statistics are in fp32 and every output is
  * rounded once, to nearest even.  Gradients use no atomics on values: the same
- * inputs give the same bits.  Outputs do not overlap inputs unless it says so.
+ * inputs give the same bits.  Outputs do not overlap inputs unless it says so, nor
+ * one another (a weight that is used twice has two gradients to add up).
  * A workspace (256-byte aligned device memory) belongs to one call at a time. */
 enum { EG_F32 = 0, EG_F16 = 1, EG_BF16 = 30 };
 /* out[t] = scale * table[ids[t]], t < n; an id outside [0, vocab) is padding and

@@ -181,3 +181,21 @@ def test_glu_grad_past_the_range_of_fp16(ops, dw):
     other, rest = torch.arange(n, device=DEV) != t, torch.arange(m, device=DEV) != c
     assert torch.equal(dx[other], want[0][other])
     assert torch.equal(dwg[rest], want[1][rest]) and torch.equal(dwu[rest], want[2][rest])
+
+
+def test_one_tensor_for_two_gradients_is_refused(ops):
+    """Queries and keys (or gate and up) that share a weight still have a gradient each."""
+    n, hq, hkv, d = 20, 2, 1, 64
+    q, k, v, w, _, cos, sin, pos, g = rows.qkv_inputs(n, hq, hkv, d, F32, F32, 3)
+    gs = [rows.randn(t.shape, g) for t in (q, k)]
+    dx, dw = [torch.full_like(t, 7.0) for t in gs], torch.full((d,), 7.0, device=DEV)
+    call = lambda a, b: ops.qkv_norm_rope_grad(*dx, None, a, b, *gs, None, q, k, None, w, w, cos, sin, pos, accumulate=True)
+    with pytest.raises(ValueError, match="same memory"):
+        call(dw, dw)
+    x, wg, _, dout = gated.inputs(20, 64, 72, BF16, 4)
+    dwg = torch.full((72, 64), 7.0, device=DEV)
+    with pytest.raises(ValueError, match="same memory"):
+        ops.glu_grad(None, dwg, dwg, dout, x, wg, wg, accumulate=True)
+    assert (dw == 7).all() and (dwg == 7).all() and all((t == 7).all() for t in dx)
+    call(dw.zero_(), torch.zeros_like(dw))  # apart: taken, with the weight itself shared
+    ops.glu_grad(None, dwg, torch.zeros_like(dwg), dout, x, wg, wg, accumulate=True)
