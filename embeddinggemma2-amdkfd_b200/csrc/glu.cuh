@@ -7,7 +7,8 @@
 //
 //   dG = dout U act'(G), dU = dout act(G)              (GLU_DGRAD: rounded once to the operands' type,
 //                                                       since the next products take them as operands)
-//                                                       (in fp16 infinite above 65504)
+//                                                       (in fp16 infinite above 65504); where they
+//                                                       are few, what that leaves is kept too)
 //   dx = dG Wg + dU Wu, dWg = dG^T x, dWu = dU^T x     (GLU_PRODUCTS)
 //
 // act is gelu_tanh(g) = g s(2 c (g + 0.044715 g^3)), c = sqrt(2/pi), or silu(g) =
@@ -68,12 +69,14 @@ struct GluCfg {
 };
 
 struct GluMaps {
-    CUtensorMap x, wg, wu, dg, du;  // dg, du: GLU_PRODUCTS only
+    CUtensorMap x, wg, wu, dg, du, dgl, dul;  // dg, du, and dgl, dul with halves = 2: GLU_PRODUCTS only
 };
 struct GluParams {
     int n, k, m;
     const void *dout;             // GLU_DGRAD
     long long dout_stride;
+    void *low[2];                 // DGRAD below 256 columns: what dG's and dU's roundings left (null: not kept)
+    int halves;                   // PRODUCTS: 2 where those are operands too, else 1
     void *out[3];                 // FORWARD: out; DGRAD: dG, dU; PRODUCTS: dx, dWg, dWu (null: not wanted)
     long long out_stride[3];
     int dw_f32, dw_accumulate;    // PRODUCTS: the weight gradients' type, and whether they are added to
@@ -148,6 +151,13 @@ __device__ __forceinline__ float glu_act_grad(float g, float *act) {
     *act = g * s;
     return s * fmaf(b * dz, 1.0f - s, 1.0f);
 }
+// What rounding a pair to T left of it, rounded to T (nothing where it became infinite).
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(float2 f, uint32_t rounded) {
+    const T *h = reinterpret_cast<const T *>(&rounded);
+    const float a = to_f32(h[0]), b = to_f32(h[1]);
+    return pack2<T>(isinf(a) ? 0.0f : f.x - a, isinf(b) ? 0.0f : f.y - b);
+}
 // ---------------------------------------------------------------- tiles
 // kind 0: the projections' tile or dx's; kinds 1 and 2: dWg's and dWu's.
 struct GluTile {
@@ -158,7 +168,7 @@ __device__ __forceinline__ GluTile glu_tile(const GluParams &p, int i) {
     const int steps_m = (p.m + 63) / 64;
     int kind = 0, rows = p.n, cols = p.m, bn = BN / 2, steps = (p.k + 63) / 64, step0 = 0, part = 0;
     if (MODE == GLU_PRODUCTS) {
-        cols = p.k, bn = BN, steps = 2 * steps_m;
+        cols = p.k, bn = BN, steps = 2 * steps_m * p.halves;
         if (i < p.dx_tiles) {
             const int each = p.dx_tiles / p.splits;
             part = i / each, i -= part * each;
@@ -166,7 +176,7 @@ __device__ __forceinline__ GluTile glu_tile(const GluParams &p, int i) {
             steps = int((long long)steps * (part + 1) / p.splits) - step0;
         } else {
             i -= p.dx_tiles;
-            rows = p.m, steps = (p.n + 63) / 64;
+            rows = p.m, steps = (p.n + 63) / 64 * p.halves;
             kind = p.out[1] ? 1 : 2;
             const int each = ((rows + 255) / 256) * ((cols + bn - 1) / bn);
             if (i >= each) i -= each, kind = 2;
@@ -245,16 +255,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<MODE, BN>::TH
                     } else {
                         const int bcol = t.col0 + rank * (BN / 2);
                         if (t.kind == 0) {
-                            const int per = (p.m + 63) / 64, ks = t.step0 + kb, seg = ks >= per, k0 = (ks - seg * per) * 64;
-                            for (int j = 0; j < 2; ++j)
-                                tma_load_2d_pair(a + j * 8192, seg ? &maps.du : &maps.dg, bar, k0, arow + j * 64);
+                            // K: dG's columns, dU's, and with two halves dG's and dU's rests.
+                            const int per = (p.m + 63) / 64, ks = t.step0 + kb;
+                            const int seg = (ks >= per) + (ks >= 2 * per) + (ks >= 3 * per), k0 = (ks - seg * per) * 64;
+                            const CUtensorMap *am = seg < 2 ? (seg ? &maps.du : &maps.dg) : seg == 2 ? &maps.dgl : &maps.dul;
+                            for (int j = 0; j < 2; ++j) tma_load_2d_pair(a + j * 8192, am, bar, k0, arow + j * 64);
                             for (int j = 0; j < BN / 128; ++j)
-                                tma_load_2d_pair(b + j * 8192, seg ? &maps.wu : &maps.wg, bar, bcol + j * 64, k0);
+                                tma_load_2d_pair(b + j * 8192, seg & 1 ? &maps.wu : &maps.wg, bar, bcol + j * 64, k0);
                         } else {
-                            for (int j = 0; j < 2; ++j)
-                                tma_load_2d_pair(a + j * 8192, t.kind == 1 ? &maps.dg : &maps.du, bar, arow + j * 64, kb * 64);
+                            // K: the tokens, and with two halves the same tokens' rests.
+                            const int per = (p.n + 63) / 64, low = kb >= per, k0 = (kb - low * per) * 64;
+                            const CUtensorMap *am = low ? (t.kind == 1 ? &maps.dgl : &maps.dul)
+                                                        : t.kind == 1 ? &maps.dg : &maps.du;
+                            for (int j = 0; j < 2; ++j) tma_load_2d_pair(a + j * 8192, am, bar, arow + j * 64, k0);
                             for (int j = 0; j < BN / 128; ++j)
-                                tma_load_2d_pair(b + j * 8192, &maps.x, bar, bcol + j * 64, kb * 64);
+                                tma_load_2d_pair(b + j * 8192, &maps.x, bar, bcol + j * 64, k0);
                         }
                     }
                 }
@@ -442,17 +457,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GluCfg<MODE, BN>::TH
                         } else {
                             float2 d[4];
                             unpack2(*place, d, T());
-                            uint32_t v[4];
+                            uint32_t v[4], wl[4], vl[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int z = 8 * j + 2 * e;
                                 float a0, a1;
                                 const float d0 = glu_act_grad<ACT>(__uint_as_float(g[z]), &a0);
                                 const float d1 = glu_act_grad<ACT>(__uint_as_float(g[z + 1]), &a1);
-                                w[e] = pack2<T>(d[e].x * __uint_as_float(u[z]) * d0, d[e].y * __uint_as_float(u[z + 1]) * d1);
-                                v[e] = pack2<T>(d[e].x * a0, d[e].y * a1);
+                                const float2 dg = make_float2(d[e].x * __uint_as_float(u[z]) * d0,
+                                                              d[e].y * __uint_as_float(u[z + 1]) * d1);
+                                const float2 du = make_float2(d[e].x * a0, d[e].y * a1);
+                                w[e] = pack2<T>(dg.x, dg.y), v[e] = pack2<T>(du.x, du.y);
+                                if (BN < 256) wl[e] = rest2<T>(dg, w[e]), vl[e] = rest2<T>(du, v[e]);
                             }
                             place[DU] = make_uint4(v[0], v[1], v[2], v[3]);
+                            if (BN < 256 && p.low[0]) {  // a few KB in all: straight from the rows' threads
+                                const int r = row0 + lane, col = t.col0 + part * (BN / 4) + c0 + 8 * j;
+                                if (r < p.n && col < p.m) {
+                                    const long long at = (long long)r * p.m + col;
+                                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.low[0]) + at) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+                                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.low[1]) + at) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
+                                }
+                            }
                         }
                         *place = make_uint4(w[0], w[1], w[2], w[3]);
                     }

@@ -57,7 +57,7 @@ static cudaError_t glu_project(const void *x, int64_t xs, const void *wg, int64_
     const int pairs = glu_pairs(), steps = ceil_div(p.k, 64);
     int bn = 256;
     long long best = LLONG_MAX;
-    for (int i = 2; i >= 0; --i) {
+    for (int i = MODE == GLU_DGRAD && p.low[0] ? 1 : 2; i >= 0; --i) {  // 256 columns have no room for the rests
         const long long c = glu_cost(glu_tiles(unsigned(p.n), unsigned(p.m), 32 << i), steps, i, pairs);
         if (c < best) best = c, bn = 64 << i;
     }
@@ -146,12 +146,16 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
     p.n = int(a.n), p.k = int(a.k), p.m = int(a.m);
     p.dout = a.dout, p.dout_stride = os;
     p.out[0] = dg, p.out[1] = du, p.out_stride[0] = p.out_stride[1] = a.m;
+    p.halves = glu_halves(a.n, a.k, a.m);
+    if (p.halves == 2) p.low[0] = du + glu_half(a.n, a.m), p.low[1] = du + 2 * glu_half(a.n, a.m);
     if (cudaError_t e = glu_project<GLU_DGRAD>(a.x, xs, a.w_gate, gs, a.w_up, us, a.type, a.act, p, s)) return e;
 
     GluMaps maps{};
     if (!glu_tmap(&maps.x, a.type, a.x, xs, a.k, a.n, 64) || !glu_tmap(&maps.wg, a.type, a.w_gate, gs, a.k, a.m, 64) ||
         !glu_tmap(&maps.wu, a.type, a.w_up, us, a.k, a.m, 64) || !glu_tmap(&maps.dg, a.type, dg, a.m, a.m, a.n, 64) ||
-        !glu_tmap(&maps.du, a.type, du, a.m, a.m, a.n, 64))
+        !glu_tmap(&maps.du, a.type, du, a.m, a.m, a.n, 64) ||
+        (p.halves == 2 && (!glu_tmap(&maps.dgl, a.type, p.low[0], a.m, a.m, a.n, 64) ||
+                           !glu_tmap(&maps.dul, a.type, p.low[1], a.m, a.m, a.n, 64))))
         return cudaErrorInvalidValue;
     p.out[0] = a.dx, p.out[1] = a.dw_gate, p.out[2] = a.dw_up;
     p.out_stride[0] = dxs, p.out_stride[1] = dgs, p.out_stride[2] = dus;
@@ -160,7 +164,7 @@ static cudaError_t glu_grad(const EgGluGrad &a, cudaStream_t s) {
     const int pairs = glu_pairs() < GLU_PAIRS ? glu_pairs() : GLU_PAIRS;
     const GluPlan plan = glu_plan(a.n, a.k, a.m, a.dx != nullptr, weights, pairs, most);
     const int w_tiles = weights * glu_tiles(a.m, a.k, 256);
-    p.splits = plan.splits, p.parts = reinterpret_cast<float *>(dg + 2 * glu_half(a.n, a.m));
+    p.splits = plan.splits, p.parts = reinterpret_cast<float *>(dg + glu_parts_at(a.n, a.k, a.m));
     p.dx_tiles = a.dx ? glu_tiles(a.n, a.k, 256) * plan.splits : 0;
     p.tiles = p.dx_tiles + w_tiles;
     p.dx_clusters = plan.dxc < p.dx_tiles ? plan.dxc : p.dx_tiles;

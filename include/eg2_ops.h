@@ -180,9 +180,10 @@ typedef struct {
  * computed again, so nothing is kept from the forward pass.  dx [n][k] (type),
  * dw_gate and dw_up [m][k] (dw_type: type or EG_F32; with accumulate, EG_F32
  * only, added to what they hold); any of the three may be null.  The
- * projections' gradients are rounded once to type between the two steps; one
- * that leaves EG_F16's range (above 65504) is infinite there, and its token's row
- * of dx and its row of dw are then not finite, so scale an fp16 loss as usual.
+ * projections' gradients are rounded once to type between the two steps (where
+ * n m < 4096 or n k < 256, what that leaves is kept too); one that leaves EG_F16's
+ * range (above 65504) is infinite there, and its token's row of dx and its row of
+ * dw are then not finite, so scale an fp16 loss as usual.
  * dout's row stride may be 0: one row for all tokens.
  * workspace: eg2_glu_grad_workspace(n, k, m) bytes. */
 typedef struct {

@@ -78,3 +78,13 @@ def test_the_whole_device_plans_without_the_bound(H):
         most = H.most_splits(n, k, m)
         for w in (0, 1, 2):
             assert H.plan_of(n, k, m, 1, w, PAIRS, most) == H.plan_of(n, k, m, 1, w, PAIRS, MOST)
+
+
+def test_few_elements_keep_their_rests(H, eg2):
+    """With few elements in the inner gradients or in dx the workspace has both parts of the former."""
+    half = lambda n, m: (2 * n * m + 255) // 256 * 256
+    for n, k, m, parts in ((1, 512, 8, 4), (1, 512, 4088, 4), (1, 512, 4096, 2), (1, 248, 8192, 4), (1, 256, 8192, 2),
+                           (511, 64, 8, 4), (512, 64, 8, 2), (63, 64, 64, 4), (64, 64, 64, 2), (31, 8, 4096, 4),
+                           (32, 8, 4096, 2)):
+        assert H.bytes(n, k, m, 1) == parts * half(n, m)
+        assert eg2._lib.load().eg2_glu_grad_workspace(n, k, m) >= parts * half(n, m)

@@ -199,3 +199,62 @@ def test_one_tensor_for_two_gradients_is_refused(ops):
     assert (dw == 7).all() and (dwg == 7).all() and all((t == 7).all() for t in dx)
     call(dw.zero_(), torch.zeros_like(dw))  # apart: taken, with the weight itself shared
     ops.glu_grad(None, dwg, torch.zeros_like(dwg), dout, x, wg, wg, accumulate=True)
+
+
+def backward_with_rests(ref, dout, dw_dtype):
+    """gated.Ref.backward with the inner gradients as a rounded value and its rounded rest:
+    what is left is half a unit of the rest, (eps / 2)^2 of the value, or half the smallest
+    subnormal."""
+    fi = torch.finfo(ref.dtype)
+    kept = lambda v: v.abs() * (fi.eps / 2) ** 2 * (1 + 1e-6) + fi.tiny * fi.eps / 2
+    d = dout.double()
+    dg, du = d * ref.u * ref.da, d * ref.a
+    eg = d.abs() * (ref.da.abs() * ref.eu + ref.u.abs() * gated.D2 * ref.eg) * 1.01 + dg.abs() * gated.REL
+    eg = eg + d.abs() * ref.u.abs() * 2.2 * gated.REL + kept(dg)
+    eu = d.abs() * gated.D1 * ref.eg * 1.01 + du.abs() * gated.REL + kept(du)
+    n, m = d.shape
+    dx = dg @ ref.wg + du @ ref.wu
+    ax = dg.abs() @ ref.wg.abs() + du.abs() @ ref.wu.abs()
+    # Twice the terms: values and rests, the latter's absolute values far below 1 % of the former's.
+    ex = eg @ ref.wg.abs() + eu @ ref.wu.abs() + ax * 1.01 * 4 * m * 2.0 ** -23 + gated.half_unit(dx, ref.dtype)
+    out = [(dx, ex)]
+    for v, e in ((dg, eg), (du, eu)):
+        w = v.T @ ref.x
+        out.append((w, e.T @ ref.x.abs() + v.abs().T @ ref.x.abs() * 1.01 * 2 * n * 2.0 ** -23
+                    + gated.half_unit(w, dw_dtype)))
+    return out
+
+
+@pytest.mark.parametrize("n,k,m", [(1, 8, 8), (1, 512, 2048), (2, 80, 392), (3, 144, 1280), (15, 72, 264), (63, 136, 64),
+                                   (64, 520, 56), (65, 64, 56), (127, 64, 32), (500, 40, 8), (1, 64, 4088), (3, 2056, 1360),
+                                   (1, 136, 6520), (3, 80, 8200), (31, 8, 520)])
+@pytest.mark.parametrize("dtype,act,dw", [(BF16, "gelu_tanh", BF16), (F16, "silu", F32), (BF16, "silu", F32)])
+def test_glu_grad_of_few_elements(ops, n, k, m, dtype, act, dw):
+    """Few elements: the inner gradients keep what their roundings left, and the results are
+    within their own rounding and 2^-16 or so, not two roundings, of the definition."""
+    assert n * m < 4096 or n * k < 256
+    x, wg, wu, dout = gated.inputs(n, k, m, dtype, n + 2 * k + m)
+    dx = torch.full((n + 3, k), 7.0, dtype=dtype, device=DEV)
+    dws = [torch.full((m + 1, k), 7.0, dtype=dw, device=DEV) for _ in range(2)]
+    ws = torch.full((ops.glu_grad_workspace(n, k, m) + 256,), 255, dtype=torch.uint8, device=DEV)  # NaN in any type
+    ops.glu_grad(dx[:n], dws[0][:m], dws[1][:m], dout, x, wg, wu, act, workspace=ws[:-256])
+    ref = backward_with_rests(gated.Ref(x, wg, wu, act, dtype), dout, dw)
+    for name, got, (r, e) in zip(("dx", "dw_gate", "dw_up"), (dx[:n], dws[0][:m], dws[1][:m]), ref):
+        gated.assert_within(got, r, e, name)
+    assert (dx[n:] == 7).all() and all((t[m:] == 7).all() for t in dws) and (ws[-256:] == 255).all()
+    for i in range(3):  # each alone: the same bits for the weights', the same bounds for dx
+        part = [None] * 3
+        part[i] = torch.full_like((dx[:n], dws[0][:m], dws[1][:m])[i], 7.0)
+        ops.glu_grad(*part, dout, x, wg, wu, act)
+        gated.assert_within(part[i], *ref[i])
+        assert i == 0 or torch.equal(part[i], dws[i - 1][:m])
+    assert ops.read_error() == 0
+
+
+def test_glu_grad_of_few_elements_past_the_range_of_fp16(ops):
+    """An inner gradient that becomes infinite leaves no rest: dw is infinite, not NaN."""
+    x, wg, wu, dout = gated.inputs(3, 64, 40, F16, 6)
+    x[1], wg[7], wu[7], dout[1, 7] = 1.0, 0.25, 0.25, 4200.0  # 67200
+    dw = torch.empty((40, 64), device=DEV)
+    ops.glu_grad(None, dw, None, dout, x, wg, wu)
+    assert (dw[7] == float("inf")).all() and dw[:7].isfinite().all() and dw[8:].isfinite().all()
