@@ -20,14 +20,17 @@ static inline long long glu_cost(long long tiles, int steps, int width, int clus
 }
 // The projections' gradients are operands of the products that follow, rounded once to
 // 16 bits; that adds as much error as the rounding of the results.  Over many
-// elements the two add up to 1.41 times the latter, over few they need not: of 700
-// calls with n m <= 40000, 59 were more than 1.5 times as far from 64 bits as a form
-// in fp32, up to 1.96 times: with few elements in dG and dU (n m), or few in dx (n k),
-// whose own rounding then varies.  There each is two operands, the rounded value and
-// what the rounding left, and the products' K is twice as long.  At 2 x 80 x 392 that
-// takes 13.6 us where one operand took 13.1, at 1 x 512 x 2048 20.6 and 17.3.
+// elements the two add up to 1.41 times the latter, over few they need not: with few
+// elements in dG and dU (n m), or few in dx (n k), whose own rounding then varies, a
+// call could be up to 1.96 times as far from 64 bits as a form in fp32.  There each
+// is two operands, the rounded value and what the rounding left, and the products' K
+// is twice as long.  The borders: dw was more than 1.5 times as far in 6 of 1757 calls
+// with n m in 4096 .. 5791 and in none of 13800 above, dx in 81 of 1711 with n k in
+// 256 .. 1023, in 9 of 1622 in 1024 .. 2047 (up to 1.55) and in 2 of 13000 above.  At
+// 2 x 80 x 392 two operands take 13.6 us where one took 13.1, at 1 x 512 x 2048 20.6
+// and 17.3.
 static inline int glu_halves(unsigned n, unsigned k, unsigned m) {
-    return uint64_t(n) * m < 4096 || uint64_t(n) * k < 256 ? 2 : 1;
+    return uint64_t(n) * m < 6144 || uint64_t(n) * k < 1024 ? 2 : 1;
 }
 
 // The backward products' plan: dx's K in `splits` parts, and `dxc` clusters for

@@ -181,7 +181,7 @@ typedef struct {
  * dw_gate and dw_up [m][k] (dw_type: type or EG_F32; with accumulate, EG_F32
  * only, added to what they hold); any of the three may be null.  The
  * projections' gradients are rounded once to type between the two steps (where
- * n m < 4096 or n k < 256, what that leaves is kept too); one that leaves EG_F16's
+ * n m < 6144 or n k < 1024, what that leaves is kept too); one that leaves EG_F16's
  * range (above 65504) is infinite there, and its token's row of dx and its row of
  * dw are then not finite, so scale an fp16 loss as usual.
  * dout's row stride may be 0: one row for all tokens.

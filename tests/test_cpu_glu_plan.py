@@ -83,8 +83,8 @@ def test_the_whole_device_plans_without_the_bound(H):
 def test_few_elements_keep_their_rests(H, eg2):
     """With few elements in the inner gradients or in dx the workspace has both parts of the former."""
     half = lambda n, m: (2 * n * m + 255) // 256 * 256
-    for n, k, m, parts in ((1, 512, 8, 4), (1, 512, 4088, 4), (1, 512, 4096, 2), (1, 248, 8192, 4), (1, 256, 8192, 2),
-                           (511, 64, 8, 4), (512, 64, 8, 2), (63, 64, 64, 4), (64, 64, 64, 2), (31, 8, 4096, 4),
-                           (32, 8, 4096, 2)):
+    for n, k, m, parts in ((1, 2048, 8, 4), (1, 2048, 6136, 4), (1, 2048, 6144, 2), (1, 1016, 8192, 4),
+                           (1, 1024, 8192, 2), (767, 64, 8, 4), (768, 64, 8, 2), (95, 64, 64, 4), (96, 64, 64, 2),
+                           (127, 8, 4096, 4), (128, 8, 4096, 2)):
         assert H.bytes(n, k, m, 1) == parts * half(n, m)
         assert eg2._lib.load().eg2_glu_grad_workspace(n, k, m) >= parts * half(n, m)
